@@ -670,6 +670,50 @@ int gi_linear_state_keyed(float* o, const void* q, long ldq, const void* k, long
                           const float* decay, float q_scale, float* state, long state_ld, int state_rows, const int* cu_seqlens,
                           const int* seq_slots, int n_seqs, int heads, int K, int V, int n_tokens, void* stream);
 
+// Beam search's choice: of every sequence's beams x vocabulary the `width` (1 to 64) largest of score + log softmax(logits), compared
+// in 64 bits, in descending order, ties to the lowest beam and then the lowest token.  logits: [seqs * beams] rows of `vocab`
+// numbers (`dtype`, row stride ld), beams 1 to 64; scores float [seqs * beams].  A logit that is no number counts as -inf; a beam
+// whose logits are all -inf, hold a +inf, or whose score is not finite offers nothing.  Outputs [seqs][width]; where there is
+// nothing left: score -inf, parent and token -1.  scratch: gi_beam_select_scratch bytes, 16-byte aligned.
+long gi_beam_select_scratch(int rows, int vocab, int width);
+int gi_beam_select(float* out_scores, int* out_parents, int* out_tokens, const void* logits, int dtype, long ld, const float* scores,
+                   int seqs, int beams, int vocab, int width, void* scratch, long scratch_bytes, void* stream);
+
+// Fixed-size states take their beams' parents' place, in place: in each of `n` tensors (host arrays of addresses and row sizes; a
+// tensor has `rows` rows one after the other) row slots[s][j] becomes what row slots[s][parents[s][j]] held before the call.  The
+// slots of a call are distinct.  A slot outside [0, rows) or a parent outside [0, beams) leaves its row as it is.  beams 1 to
+// 64; unit 16, 4 or 1: bytes that every address and row size is a multiple of.
+int gi_reorder_states(void* const* states, const long* row_bytes, int n, int unit, const int* slots, const int* parents, int seqs,
+                      int beams, int rows, void* stream);
+
+// The first rows[i] (null: all 64) positions of page src[i] are copied to page dst[i] for every layer and head of `n` (at most 8)
+// tensors [layers][pages][heads][64][row bytes] (host arrays).  No page that is written is read or written twice in one call.
+// Pages outside a tensor are passed over.
+int gi_copy_pages(void* const* tensors, const int* layers, const int* pages, const int* heads, const int* row_bytes, int n,
+                  const int* src, const int* dst, const int* rows, int copies, void* stream);
+
+// Attention of drafted tokens: the tokens of sequence b (cu_seqlens, at most max_nodes <= 256 of them, the rest is left out) are the
+// nodes of a tree whose keys and values lie at the positions seq_pos0[b] + node of the cache already; a node sees every position
+// before seq_pos0[b] and the nodes in its row of `masks` ([tokens][words] 32-bit words, bit i of word w: node 32 w + i).  A node
+// that sees nothing gets zeros.  max_kv_len (cached positions and nodes of the longest sequence) and max_nodes size the launch; a
+// max_kv_len that is too small costs time only.  hd 1 to 256, n_seqs at most 1024.  scratch: gi_attn_tree_scratch bytes, 16-byte
+// aligned.  Keys and values of nodes that nobody sees, and what lies behind the last node, may hold anything.
+long gi_attn_tree_scratch(int n_seqs, int max_nodes, int max_kv_len, int n_heads, int n_kv, int hd, int dtype);
+int gi_attn_tree(void* out, long ldo, const void* q, long ldq, int dtype, const void* kcache, const void* vcache, int cache_pages,
+                 const int* block_table, int max_pages, const int* cu_seqlens, const int* seq_slots, const int* seq_pos0, const int* masks,
+                 int words, int n_seqs, int max_nodes, int max_kv_len, int n_heads, int n_kv, int hd, float scale, void* scratch,
+                 long scratch_bytes, void* stream);
+
+// The walk through every sequence's tree of drafted tokens: from node 0 to the first child (a later node whose entry in `parents`
+// is this node) whose token is the node's pick, as long as there is one.  out_path [n_seqs][max_nodes]: the accepted nodes, then -1;
+// out_counts; out_next: the last accepted node's pick (-1 for no nodes).  The accepted nodes' rows move from position
+// seq_pos0 + node to seq_pos0 + place in the path, in every layer and head of `n` (0 to 8) tensors of pages (as gi_copy_pages).
+// A slot of -1 moves nothing; positions outside the table or pages outside a tensor are passed over.  max_nodes 1 to 256.
+int gi_tree_commit(int* out_path, int* out_counts, int* out_next, const int* picks, const int* tokens, const int* parents,
+                   const int* cu_seqlens, const int* seq_slots, const int* seq_pos0, int n_seqs, int max_nodes, void* const* tensors,
+                   const int* layers, const int* pages, const int* heads, const int* row_bytes, int n, const int* block_table,
+                   int max_pages, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

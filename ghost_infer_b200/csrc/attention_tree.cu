@@ -1,0 +1,360 @@
+// Attention of drafted tokens over the paged cache: the nodes of one tree per sequence, each of which sees all positions cached
+// before the tree and those nodes that its mask names (its ancestors and itself, as a rule).
+//
+//     o_i = sum_t exp(scale q_i k_t - m) v_t / sum_t exp(scale q_i k_t - m)    over the keys t that node i sees
+//
+// with the running maximum m and the sums in 32 bits; a node that sees nothing gets zeros.  Keys and values of the step's own
+// nodes are in the cache already, at the positions behind the cached ones in the nodes' order.
+//
+// This file: the form on CUDA cores for 32-bit rows and for head sizes that the tensor-core form (attention_tree_t5.cu) does not
+// take, the joining of partial results, and the entry point.  A block takes up to 16 or 64 query rows (nodes x heads of a kv
+// head's group, which share every key and value that is read) and a range of tiles of 64 keys (attention_tree.cuh).  Scores are a
+// register tile of R / 16 rows by 4 keys a thread, sums of values R / 16 rows by 4 numbers for every 64 of the head; a row's 16
+// threads are one half of a warp, so its maximum and sum need no barrier.
+// Bound: 32-bit multiply-adds (4 per query number, key and value) with many rows, the cache's bytes with few.
+#include "api.h"
+#include "attention_tree.cuh"
+
+namespace {
+
+using namespace gi::tree;
+
+constexpr int THREADS = 256;
+
+template <typename T, int R, int DCH>
+__global__ void __launch_bounds__(THREADS)
+attn_tree_kernel(const Shape sh, T* __restrict__ out, long ldo, const T* q, long ldq, const T* kcache, const T* vcache, int cache_pages, int hd, float scale,
+                 int least, float* __restrict__ part_o, float* __restrict__ part_ml, long* __restrict__ part_prefix, int vec) {
+  constexpr int RT = R / 16;                       // rows a thread works on: ty + 16 i
+  extern __shared__ __align__(16) float smem[];
+  const int hp = (hd + 3) / 4 * 4, ld = hp + 4;    // rows padded: 16 rows' four-number reads fall into different banks
+  float* Qs = smem;                                // [R][ld]
+  float* Ks = Qs + R * ld;                         // [64][ld]
+  float* Vs = Ks + TILE * ld;                      // [64][ld]
+  float* Ps = Vs + TILE * ld;                      // [R][68]
+  __shared__ long s_pre[MAX_SEQS + 1];
+  const int tid = threadIdx.x, ty = tid >> 4, tx = tid & 15;
+  gi::pdl_prologue();
+  if (tid < 32) prefix(sh, s_pre);
+  __syncthreads();
+  const long total = s_pre[sh.n_seqs], per = per_block(total, gridDim.x, least);
+  if (blockIdx.x == 0)
+    for (int i = tid; i <= sh.n_seqs; i += THREADS) part_prefix[i] = s_pre[i];
+  const long lo = (long)blockIdx.x * per, hi = min(total, lo + per);
+  const int group = sh.n_heads / sh.n_kv;
+
+  for (long at = lo; at < hi;) {
+    const Unit u = unit_at(sh, s_pre, at);
+    const int t_begin = (int)(at - u.first), t_end = (int)min((long)u.tiles, hi - u.first);
+    const int tok0 = sh.cu_seqlens[u.b], len = u.pos0 + u.n;
+    const int rows_here = min(sh.rows_block, u.n * group - u.row0);
+    __syncthreads();
+    for (int i = tid; i < R * hp; i += THREADS) {
+      const int r = i / hp, d = i % hp, row = u.row0 + r;
+      Qs[r * ld + d] = r < rows_here && d < hd ? gi::ldf(q + (size_t)(tok0 + row / group) * ldq + (size_t)(u.kvh * group + row % group) * hd + d) : 0.f;
+    }
+    float m[RT], l[RT], acc[RT][DCH * 4];
+#pragma unroll
+    for (int i = 0; i < RT; ++i) {
+      m[i] = -INFINITY, l[i] = 0.f;
+#pragma unroll
+      for (int c = 0; c < DCH * 4; ++c) acc[i][c] = 0.f;
+    }
+    for (int t = t_begin; t < t_end; ++t) {
+      const int kt = t * TILE;
+      const int page = page_of(sh, u.slot, t, cache_pages);
+      const size_t base = ((size_t)page * sh.n_kv + u.kvh) * TILE * hd;
+      __syncthreads();
+      if (vec) {
+        const int h4 = hd / 4;
+        for (int i0 = tid; i0 < TILE * h4; i0 += 4 * THREADS) {
+          float4 kx[4], vx[4];
+#pragma unroll
+          for (int w = 0; w < 4; ++w) {
+            const int i = i0 + w * THREADS, r = i / h4;
+            const bool live = r < TILE && kt + r < len;       // rows past the last node are not read
+            kx[w] = live ? gi::ld4(kcache + base + (size_t)i * 4) : make_float4(0.f, 0.f, 0.f, 0.f);
+            vx[w] = live ? gi::ld4(vcache + base + (size_t)i * 4) : make_float4(0.f, 0.f, 0.f, 0.f);
+          }
+#pragma unroll
+          for (int w = 0; w < 4; ++w) {
+            const int i = i0 + w * THREADS, r = i / h4, c = i - r * h4;
+            if (r < TILE) {
+              *reinterpret_cast<float4*>(Ks + r * ld + 4 * c) = kx[w];
+              *reinterpret_cast<float4*>(Vs + r * ld + 4 * c) = vx[w];
+            }
+          }
+        }
+      } else {
+        for (int i = tid; i < TILE * hp; i += THREADS) {
+          const int r = i / hp, d = i % hp;
+          const bool live = kt + r < len && d < hd;
+          Ks[r * ld + d] = live ? gi::ldf(kcache + base + (size_t)r * hd + d) : 0.f;
+          Vs[r * ld + d] = live ? gi::ldf(vcache + base + (size_t)r * hd + d) : 0.f;
+        }
+      }
+      __syncthreads();
+      float s[RT][4];
+#pragma unroll
+      for (int i = 0; i < RT; ++i)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) s[i][j] = 0.f;
+#pragma unroll 4
+      for (int d = 0; d < hp; d += 4) {
+        float4 k4[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) k4[j] = *reinterpret_cast<const float4*>(Ks + (tx + 16 * j) * ld + d);
+#pragma unroll
+        for (int i = 0; i < RT; ++i) {
+          const float4 q4 = *reinterpret_cast<const float4*>(Qs + (ty + 16 * i) * ld + d);
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            s[i][j] = fmaf(q4.x, k4[j].x, s[i][j]);
+            s[i][j] = fmaf(q4.y, k4[j].y, s[i][j]);
+            s[i][j] = fmaf(q4.z, k4[j].z, s[i][j]);
+            s[i][j] = fmaf(q4.w, k4[j].w, s[i][j]);
+          }
+        }
+      }
+      const bool in_tree = kt + TILE > u.pos0;
+#pragma unroll
+      for (int i = 0; i < RT; ++i) {
+        const int r = ty + 16 * i;
+        unsigned seen[2] = {0xffffffffu, 0xffffffffu};
+        if (in_tree) {
+          const int* mask = sh.masks + (size_t)(tok0 + min(u.row0 + r, u.n * group - 1) / group) * sh.words;
+          seen[0] = seen_word(mask, sh.words, u.n, kt - u.pos0);
+          seen[1] = seen_word(mask, sh.words, u.n, kt + 32 - u.pos0);
+        }
+        float top = -INFINITY;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const int key = tx + 16 * j;
+          s[i][j] = (seen[j >> 1] >> (key & 31)) & 1u ? s[i][j] * scale : -INFINITY;
+          top = fmaxf(top, s[i][j]);
+        }
+#pragma unroll
+        for (int o = 8; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+        const float m_new = fmaxf(m[i], top), ref = m_new == -INFINITY ? 0.f : m_new;
+        const float alpha = m[i] == -INFINITY ? 0.f : expf(m[i] - ref);
+        m[i] = m_new;
+        float sum = 0.f;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const float p = expf(s[i][j] - ref);
+          sum += p;
+          Ps[r * 68 + tx + 16 * j] = p;
+        }
+#pragma unroll
+        for (int o = 8; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+        l[i] = l[i] * alpha + sum;
+#pragma unroll
+        for (int c = 0; c < DCH * 4; ++c) acc[i][c] *= alpha;
+      }
+      __syncwarp();
+      // a node's value that is no number must not reach those that do not see the node: a weight of zero takes nothing
+      for (int j = 0; j < TILE; j += 4) {
+        float4 v4[4][DCH];
+#pragma unroll
+        for (int w = 0; w < 4; ++w)
+#pragma unroll
+          for (int c = 0; c < DCH; ++c)
+            if (c * 64 + tx * 4 < hp) v4[w][c] = *reinterpret_cast<const float4*>(Vs + (j + w) * ld + c * 64 + tx * 4);
+#pragma unroll
+        for (int i = 0; i < RT; ++i) {
+          const float4 p4 = *reinterpret_cast<const float4*>(Ps + (ty + 16 * i) * 68 + j);
+          const float p[4] = {p4.x, p4.y, p4.z, p4.w};
+#pragma unroll
+          for (int w = 0; w < 4; ++w) {
+            if (in_tree && p[w] == 0.f) continue;
+#pragma unroll
+            for (int c = 0; c < DCH; ++c)
+              if (c * 64 + tx * 4 < hp) {
+                acc[i][c * 4] = fmaf(p[w], v4[w][c].x, acc[i][c * 4]);
+                acc[i][c * 4 + 1] = fmaf(p[w], v4[w][c].y, acc[i][c * 4 + 1]);
+                acc[i][c * 4 + 2] = fmaf(p[w], v4[w][c].z, acc[i][c * 4 + 2]);
+                acc[i][c * 4 + 3] = fmaf(p[w], v4[w][c].w, acc[i][c * 4 + 3]);
+              }
+          }
+        }
+      }
+    }
+    const bool whole = t_begin == 0 && t_end == u.tiles;
+    const size_t slot2 = 2 * (size_t)blockIdx.x + (t_begin == 0 ? 1 : 0);
+#pragma unroll
+    for (int i = 0; i < RT; ++i) {
+      const int r = ty + 16 * i;
+      if (r >= rows_here) continue;
+      const int row = u.row0 + r;
+      T* dst = out + (size_t)(tok0 + row / group) * ldo + (size_t)(u.kvh * group + row % group) * hd;
+      const float inv = l[i] == 0.f ? 0.f : 1.0f / l[i];
+#pragma unroll
+      for (int c = 0; c < DCH * 4; ++c) {
+        const int d = (c / 4) * 64 + tx * 4 + (c & 3);
+        if (d >= hd) continue;
+        if (whole) gi::stf(dst + d, acc[i][c] * inv);
+        else part_o[(slot2 * sh.rows_block + r) * hd + d] = acc[i][c];
+      }
+      if (!whole && tx == 0) {
+        part_ml[(slot2 * sh.rows_block + r) * 2] = m[i];
+        part_ml[(slot2 * sh.rows_block + r) * 2 + 1] = l[i];
+      }
+    }
+    at = u.first + t_end;
+  }
+}
+
+// Joins the parts of the units that several blocks hold; maxima are in units of ln (base 1) or of powers of two (base2).  A warp
+// takes a row's parts, or, where a row may have many, all warps of a block do and meet in shared memory.
+template <typename T, bool SHARED_ROWS>
+__global__ void __launch_bounds__(THREADS)
+attn_tree_join_kernel(const Shape sh, T* __restrict__ out, long ldo, int hd, int blocks, int least, int base2, const float* part_o, const float* part_ml,
+                      const long* part_prefix) {
+  constexpr int WARPS = THREADS / 32, NUMBERS = 8;         // numbers of a head per lane: head sizes up to 256
+  __shared__ float s_acc[SHARED_ROWS ? WARPS : 1][256];
+  __shared__ float s_l[WARPS];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  gi::pdl_prologue();
+  const int b = blockIdx.z, kvh = blockIdx.y, group = sh.n_heads / sh.n_kv;
+  const int row = SHARED_ROWS ? blockIdx.x : blockIdx.x * WARPS + warp;
+  const int n = nodes_of(sh, b);
+  if (row >= n * group) return;                            // (a block's rows: the same for all of a block that meets)
+  const long total = part_prefix[sh.n_seqs], per = per_block(total, blocks, least);
+  const int tiles = (pos0_of(sh, b) + n + TILE - 1) / TILE;
+  const long first = part_prefix[b] + ((long)(row / sh.rows_block) * sh.n_kv + kvh) * tiles;
+  const int c0 = (int)(first / per), c1 = (int)((first + tiles - 1) / per);
+  if (c0 == c1) return;                                    // one block had it all
+  const int r = row % sh.rows_block;
+  auto slot_of = [&](int c) { return (2 * (size_t)c + (c == c0 ? 1 : 0)) * sh.rows_block + r; };
+  float m = -INFINITY, l = 0.f, acc[NUMBERS];
+#pragma unroll
+  for (int i = 0; i < NUMBERS; ++i) acc[i] = 0.f;
+  for (int c = c0 + lane; c <= c1; c += 32) m = fmaxf(m, part_ml[slot_of(c) * 2]);
+  m = gi::warp_max(m);
+  const float ref = m == -INFINITY ? 0.f : m;
+#pragma unroll 2
+  for (int c = c0 + (SHARED_ROWS ? warp : 0); c <= c1; c += SHARED_ROWS ? WARPS : 1) {
+    const size_t s = slot_of(c);
+    const float pm = part_ml[s * 2], pl = part_ml[s * 2 + 1];
+    const float w = base2 ? exp2f(pm - ref) : expf(pm - ref);
+    l += w * pl;
+#pragma unroll
+    for (int i = 0; i < NUMBERS; ++i)
+      if (lane + 32 * i < hd) {
+        const float o = part_o[s * hd + lane + 32 * i];
+        if (w != 0.f) acc[i] = fmaf(w, o, acc[i]);
+      }
+  }
+  T* dst = out + (size_t)(sh.cu_seqlens[b] + row / group) * ldo + (size_t)(kvh * group + row % group) * hd;
+  if (SHARED_ROWS) {
+#pragma unroll
+    for (int i = 0; i < NUMBERS; ++i) s_acc[warp][lane + 32 * i] = acc[i];
+    if (lane == 0) s_l[warp] = l;
+    __syncthreads();
+    l = 0.f;
+    for (int w = 0; w < WARPS; ++w) l += s_l[w];
+    const float inv = l == 0.f ? 0.f : 1.0f / l;
+    for (int d = threadIdx.x; d < hd; d += THREADS) {
+      float o = 0.f;
+      for (int w = 0; w < WARPS; ++w) o += s_acc[w][d];
+      gi::stf(dst + d, o * inv);
+    }
+    return;
+  }
+  const float inv = l == 0.f ? 0.f : 1.0f / l;
+#pragma unroll
+  for (int i = 0; i < NUMBERS; ++i)
+    if (lane + 32 * i < hd) gi::stf(dst + lane + 32 * i, acc[i] * inv);
+}
+
+struct Plan {
+  int blocks, least, rows_block;
+  bool wide_rows;       // 64 query rows a block
+  bool many_parts;      // a unit may lie on more blocks than one warp should join
+};
+
+constexpr int LEAST_TILES = 2;
+
+// A row block of whole nodes; one unit's tiles go to one block only where there are more units than blocks.
+Plan plan_of(int n_seqs, int max_nodes, int max_kv_len, int n_heads, int n_kv) {
+  Plan p;
+  const int group = n_heads / n_kv;
+  const long rows = (long)max_nodes * group;
+  p.wide_rows = rows > 16;
+  const int most = p.wide_rows ? 64 : 16;
+  p.rows_block = most;
+  const long units = (long)n_seqs * n_kv * ((rows + most - 1) / most), tiles = (max_kv_len + TILE - 1) / TILE;
+  p.least = LEAST_TILES;
+  const long wanted = units * ((tiles + p.least - 1) / p.least);
+  const long cap = 2L * gi::sm_count();
+  p.blocks = (int)(wanted < cap ? (wanted > 1 ? wanted : 1) : cap);
+  p.many_parts = p.blocks > 16 * units;
+  return p;
+}
+
+template <typename T, int R, int DCH>
+int launch_tree(const Shape& sh, const Plan& p, T* out, long ldo, const T* q, long ldq, const T* k, const T* v, int cache_pages, int hd, float scale,
+                float* part_o, float* part_ml, long* part_prefix, cudaStream_t s) {
+  const int hp = (hd + 3) / 4 * 4;
+  const size_t smem = ((size_t)(R + 2 * TILE) * (hp + 4) + (size_t)R * 68) * sizeof(float);
+  auto kern = attn_tree_kernel<T, R, DCH>;
+  static bool configured[gi::MAX_DEVICES_SEEN] = {false};
+  int dev;
+  if (gi::unconfigured_here(configured, &dev)) {
+    const size_t most = ((size_t)(R + 2 * TILE) * (DCH * 64 + 4) + (size_t)R * 68) * sizeof(float);
+    cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)most);
+    if (e != cudaSuccess) return gi::fail(GI_ERR_CUDA, "tree attention: %s", cudaGetErrorString(e));
+    if (dev >= 0) configured[dev] = true;
+  }
+  const int vec = hd % 4 == 0 && ((uintptr_t)k % (4 * sizeof(T))) == 0 && ((uintptr_t)v % (4 * sizeof(T))) == 0;
+  return gi::check(gi::launch(kern, dim3(p.blocks), dim3(THREADS), smem, s, sh, out, ldo, q, ldq, k, v, cache_pages, hd, scale, p.least, part_o, part_ml,
+                              part_prefix, vec), "tree attention");
+}
+
+template <typename T, int R>
+int launch_tree_dims(const Shape& sh, const Plan& p, T* out, long ldo, const T* q, long ldq, const T* k, const T* v, int cache_pages, int hd, float scale,
+                     float* part_o, float* part_ml, long* part_prefix, cudaStream_t s) {
+  if (hd <= 64) return launch_tree<T, R, 1>(sh, p, out, ldo, q, ldq, k, v, cache_pages, hd, scale, part_o, part_ml, part_prefix, s);
+  if (hd <= 128) return launch_tree<T, R, 2>(sh, p, out, ldo, q, ldq, k, v, cache_pages, hd, scale, part_o, part_ml, part_prefix, s);
+  return launch_tree<T, R, 4>(sh, p, out, ldo, q, ldq, k, v, cache_pages, hd, scale, part_o, part_ml, part_prefix, s);
+}
+
+}  // namespace
+
+extern "C" long gi_attn_tree_scratch(int n_seqs, int max_nodes, int max_kv_len, int n_heads, int n_kv, int hd, int dtype) {
+  if (n_seqs <= 0 || max_nodes <= 0 || max_kv_len <= 0 || n_kv <= 0 || n_heads < n_kv || hd <= 0) return 0;
+  const Plan p = plan_of(n_seqs, max_nodes, max_kv_len, n_heads, n_kv);
+  return 8L * (n_seqs + 2) + 2L * p.blocks * p.rows_block * (hd + 2) * 4;
+}
+
+extern "C" int gi_attn_tree(void* out, long ldo, const void* q, long ldq, int dtype, const void* kcache, const void* vcache, int cache_pages,
+                            const int* block_table, int max_pages, const int* cu_seqlens, const int* seq_slots, const int* seq_pos0, const int* masks,
+                            int words, int n_seqs, int max_nodes, int max_kv_len, int n_heads, int n_kv, int hd, float scale, void* scratch,
+                            long scratch_bytes, void* stream) {
+  if (n_seqs <= 0) return GI_OK;
+  if (n_kv < 1 || n_heads < 1 || n_heads % n_kv != 0) return gi::fail(GI_ERR_ARG, "tree attention: %d heads do not divide into %d kv heads", n_heads, n_kv);
+  if (hd < 1 || hd > 256) return gi::fail(GI_ERR_UNSUPPORTED, "tree attention: head size %d, 1 to 256 are supported", hd);
+  if (max_nodes < 1 || max_nodes > MAX_NODES) return gi::fail(GI_ERR_ARG, "tree attention: trees of up to %d nodes, 1 to %d are supported", max_nodes, MAX_NODES);
+  if (words < (max_nodes + 31) / 32) return gi::fail(GI_ERR_ARG, "tree attention: %d words of mask bits cannot hold %d nodes", words, max_nodes);
+  if (n_seqs > MAX_SEQS) return gi::fail(GI_ERR_UNSUPPORTED, "tree attention: more than %d sequences in one launch", MAX_SEQS);
+  if (cache_pages < 1 || max_pages < 1 || max_kv_len < 1) return gi::fail(GI_ERR_ARG, "tree attention: %d pages, %d in a table's row, %d positions", cache_pages, max_pages, max_kv_len);
+  const Plan p = plan_of(n_seqs, max_nodes, max_kv_len, n_heads, n_kv);
+  if (scratch_bytes < gi_attn_tree_scratch(n_seqs, max_nodes, max_kv_len, n_heads, n_kv, hd, dtype) || ((uintptr_t)scratch & 15))
+    return gi::fail(GI_ERR_ARG, "tree attention: the scratch memory is too small or not aligned");
+  Shape sh = {cu_seqlens, seq_slots, seq_pos0, block_table, masks, words, max_pages, n_seqs, n_heads, n_kv, p.rows_block, max_nodes};
+  long* prefix_out = (long*)scratch;
+  float* part_o = (float*)(prefix_out + (n_seqs + 2) / 2 * 2);
+  float* part_ml = part_o + 2L * p.blocks * p.rows_block * hd;
+  cudaStream_t s = (cudaStream_t)stream;
+  int rc = GI_OK;
+  if (p.wide_rows)
+    GI_DISPATCH_DTYPE(dtype, T, rc = (launch_tree_dims<T, 64>(sh, p, (T*)out, ldo, (const T*)q, ldq, (const T*)kcache, (const T*)vcache, cache_pages, hd, scale, part_o, part_ml, prefix_out, s)));
+  else
+    GI_DISPATCH_DTYPE(dtype, T, rc = (launch_tree_dims<T, 16>(sh, p, (T*)out, ldo, (const T*)q, ldq, (const T*)kcache, (const T*)vcache, cache_pages, hd, scale, part_o, part_ml, prefix_out, s)));
+  if (rc != GI_OK) return rc;
+  const int rows = max_nodes * (n_heads / n_kv);
+  const dim3 join(p.many_parts ? rows : (rows + 7) / 8, n_kv, n_seqs);
+  GI_DISPATCH_DTYPE(dtype, T, rc = gi::check(gi::launch(p.many_parts ? attn_tree_join_kernel<T, true> : attn_tree_join_kernel<T, false>, join, dim3(THREADS), 0, s, sh,
+                                                        (T*)out, ldo, hd, p.blocks, p.least, 0, part_o, part_ml, prefix_out), "tree attention (join)"));
+  return rc;
+}

@@ -1,0 +1,145 @@
+// What a step over trees of drafted tokens leaves behind: the walk through each tree as far as the model's picks agree, and the
+// accepted tokens' keys and values moved up to follow the cache directly.
+//
+// A sequence's nodes were stored at the positions pos0, pos0 + 1, ... in their order (a node comes after its parent), node 0
+// being the token that would have been fed anyway.  The walk starts there; from a node it goes to the first of its children
+// whose token is what the model picks at the node, and ends where there is none.  The accepted nodes, in the order of the
+// walk, get positions pos0, pos0 + 1, ...: node path[i] moves to pos0 + i.  path[i] >= i and the path ascends, so no move
+// overwrites what a later one reads; a thread that moves its column of 2 to 16 bytes of every accepted row in the path's order
+// needs nobody to wait for.
+// Every block repeats the walk over its sequence's nodes in shared memory (one warp, a round of the nodes per accepted one): that
+// costs less than a launch of its own that the moves would wait for.  Bound: latency; the moved rows' bytes for many sequences.
+#include "api.h"
+#include "common.cuh"
+
+namespace {
+
+constexpr int THREADS = 256;
+constexpr int MAX_NODES = 256;
+constexpr int MAX_PAGE_TENSORS = 8;
+
+struct TreeTensors {
+  void* base[MAX_PAGE_TENSORS];
+  int layers[MAX_PAGE_TENSORS], pages[MAX_PAGE_TENSORS], heads[MAX_PAGE_TENSORS], row_units[MAX_PAGE_TENSORS];
+  long columns[MAX_PAGE_TENSORS];    // layers * heads * row units
+};
+
+template <typename V>
+__global__ void __launch_bounds__(THREADS)
+tree_commit_kernel(const __grid_constant__ TreeTensors t, int n_tensors, const int* picks, const int* tokens, const int* parents,
+                   const int* cu_seqlens, const int* seq_slots, const int* seq_pos0, const int* block_table, int max_pages, int max_nodes,
+                   int* __restrict__ out_path, int* __restrict__ out_counts, int* __restrict__ out_next) {
+  __shared__ int s_token[MAX_NODES], s_parent[MAX_NODES], s_pick[MAX_NODES], s_path[MAX_NODES], s_page[MAX_NODES / PAGE_TOKENS + 2];
+  __shared__ int s_count;
+  const int tid = threadIdx.x, lane = tid & 31, b = blockIdx.y;
+  gi::pdl_prologue();
+  const int tok0 = cu_seqlens[b], n = min(cu_seqlens[b + 1] - tok0, max_nodes);
+  const int slot = seq_slots[b], pos0 = seq_pos0[b];
+  for (int i = tid; i < n; i += THREADS) {
+    s_token[i] = tokens[tok0 + i];
+    s_parent[i] = parents[tok0 + i];
+    s_pick[i] = picks[tok0 + i];
+  }
+  const int page0 = pos0 / PAGE_TOKENS, n_pages = MAX_NODES / PAGE_TOKENS + 2;
+  for (int i = tid; i < n_pages; i += THREADS)
+    s_page[i] = slot >= 0 && pos0 >= 0 && page0 + i < max_pages ? block_table[(size_t)slot * max_pages + page0 + i] : -1;
+  __syncthreads();
+  if (tid < 32) {
+    int count = 0, at = 0;
+    bool on = n > 0;
+    while (on) {                              // (ascends: at most n rounds)
+      if (lane == 0) s_path[count] = at;
+      ++count;
+      const int pick = s_pick[at];
+      int next = n;
+      for (int i0 = at + 1; i0 < n && next == n; i0 += 32) {
+        const int i = i0 + lane;
+        const unsigned who = __ballot_sync(0xffffffffu, i < n && s_parent[i] == at && s_token[i] == pick);
+        if (who) next = i0 + __ffs(who) - 1;
+      }
+      on = next < n;
+      if (on) at = next;
+    }
+    if (lane == 0) {
+      s_count = count;
+      if (blockIdx.x == 0) {
+        out_counts[b] = count;
+        out_next[b] = count > 0 ? s_pick[at] : -1;
+      }
+    }
+  }
+  __syncthreads();
+  const int count = s_count;
+  if (blockIdx.x == 0)
+    for (int i = tid; i < max_nodes; i += THREADS) out_path[(size_t)b * max_nodes + i] = i < count ? s_path[i] : -1;
+  int first = 0;                              // what is in its place already
+  while (first < count && s_path[first] == first) ++first;
+  if (first >= count) return;
+
+  long col = (long)blockIdx.x * THREADS + tid;
+  int z = 0;
+  while (z < n_tensors && col >= t.columns[z]) col -= t.columns[z++];
+  if (z >= n_tensors) return;
+  const int ru = t.row_units[z], c = (int)(col % ru), head = (int)(col / ru % t.heads[z]), layer = (int)(col / ru / t.heads[z]);
+  V* base = (V*)t.base[z];
+  const int off0 = pos0 % PAGE_TOKENS;
+  auto place = [&](int i) -> V* {             // the column's place of position pos0 + i; null outside the cache
+    const int page = s_page[(off0 + i) / PAGE_TOKENS];
+    if (page < 0 || page >= t.pages[z]) return nullptr;
+    return base + ((((size_t)layer * t.pages[z] + page) * t.heads[z] + head) * PAGE_TOKENS + (off0 + i) % PAGE_TOKENS) * ru + c;
+  };
+  constexpr int AHEAD = 8;
+  for (int i0 = first; i0 < count; i0 += AHEAD) {
+    V held[AHEAD];
+    bool ok[AHEAD];
+#pragma unroll
+    for (int k = 0; k < AHEAD; ++k) {
+      ok[k] = i0 + k < count;
+      if (ok[k]) {
+        const V* from = place(s_path[i0 + k]);
+        ok[k] = from != nullptr;
+        if (ok[k]) held[k] = *from;
+      }
+    }
+#pragma unroll
+    for (int k = 0; k < AHEAD; ++k)
+      if (ok[k]) {
+        V* to = place(i0 + k);
+        if (to != nullptr) *to = held[k];
+      }
+  }
+}
+
+}  // namespace
+
+extern "C" int gi_tree_commit(int* out_path, int* out_counts, int* out_next, const int* picks, const int* tokens, const int* parents,
+                              const int* cu_seqlens, const int* seq_slots, const int* seq_pos0, int n_seqs, int max_nodes, void* const* tensors,
+                              const int* layers, const int* pages, const int* heads, const int* row_bytes, int n, const int* block_table,
+                              int max_pages, void* stream) {
+  if (n_seqs <= 0) return GI_OK;
+  if (max_nodes < 1 || max_nodes > MAX_NODES) return gi::fail(GI_ERR_ARG, "tree commit: trees of up to %d nodes, 1 to %d are supported", max_nodes, MAX_NODES);
+  if (n_seqs > 65535) return gi::fail(GI_ERR_UNSUPPORTED, "tree commit: more than 65535 sequences in one launch");
+  if (n < 0 || n > MAX_PAGE_TENSORS) return gi::fail(GI_ERR_UNSUPPORTED, "tree commit: %d tensors of pages, at most %d in one launch", n, MAX_PAGE_TENSORS);
+  int unit = 16;
+  for (int i = 0; i < n; ++i) {
+    if (layers[i] < 1 || pages[i] < 1 || heads[i] < 1 || row_bytes[i] < 2 || row_bytes[i] % 2 != 0 || ((uintptr_t)tensors[i] & 1))
+      return gi::fail(GI_ERR_ARG, "tree commit: tensor %d has %d layers, %d pages, %d heads, rows of %d bytes", i, layers[i], pages[i], heads[i], row_bytes[i]);
+    while (unit > 2 && (row_bytes[i] % unit != 0 || ((uintptr_t)tensors[i] % unit) != 0)) unit = unit == 16 ? 4 : 2;
+  }
+  TreeTensors t = {};
+  long columns = 0;
+  for (int i = 0; i < n; ++i) {
+    t.base[i] = tensors[i], t.layers[i] = layers[i], t.pages[i] = pages[i], t.heads[i] = heads[i], t.row_units[i] = row_bytes[i] / unit;
+    columns += t.columns[i] = (long)layers[i] * heads[i] * (row_bytes[i] / unit);
+  }
+  const long blocks = columns > 0 ? (columns + THREADS - 1) / THREADS : 1;
+  if (blocks > 0x7fffffffL) return gi::fail(GI_ERR_UNSUPPORTED, "tree commit: more rows' columns than one launch holds");
+  const dim3 grid((unsigned)blocks, n_seqs);
+  cudaStream_t s = (cudaStream_t)stream;
+#define GI_TREE(V) gi::check(gi::launch(tree_commit_kernel<V>, grid, dim3(THREADS), 0, s, t, n, picks, tokens, parents, cu_seqlens, seq_slots, seq_pos0, \
+                                        block_table, max_pages, max_nodes, out_path, out_counts, out_next), "tree commit")
+  if (unit == 16) return GI_TREE(uint4);
+  if (unit == 4) return GI_TREE(unsigned);
+  return GI_TREE(unsigned short);
+#undef GI_TREE
+}
