@@ -703,6 +703,8 @@ int gi_attn_tree(void* out, long ldo, const void* q, long ldq, int dtype, const 
                  const int* block_table, int max_pages, const int* cu_seqlens, const int* seq_slots, const int* seq_pos0, const int* masks,
                  int words, int n_seqs, int max_nodes, int max_kv_len, int n_heads, int n_kv, int hd, float scale, void* scratch,
                  long scratch_bytes, void* stream);
+// Nonzero: a bounded wait of the tensor-core form ran out since the last question (and asks for it once).
+int gi_attn_tree_status(int* status);
 
 // The walk through every sequence's tree of drafted tokens: from node 0 to the first child (a later node whose entry in `parents`
 // is this node) whose token is the node's pick, as long as there is one.  out_path [n_seqs][max_nodes]: the accepted nodes, then -1;

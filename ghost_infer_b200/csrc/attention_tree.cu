@@ -269,28 +269,27 @@ attn_tree_join_kernel(const Shape sh, T* __restrict__ out, long ldo, int hd, int
 
 struct Plan {
   int blocks, least, rows_block;
-  bool wide_rows;       // 64 query rows a block
   bool many_parts;      // a unit may lie on more blocks than one warp should join
 };
 
 constexpr int LEAST_TILES = 2;
 
-// A row block of whole nodes; one unit's tiles go to one block only where there are more units than blocks.
-Plan plan_of(int n_seqs, int max_nodes, int max_kv_len, int n_heads, int n_kv) {
+// The query rows of a block: 16 or 64 on CUDA cores, 128 or 256 on tensor cores, the smaller where it holds a tree's rows; blocks:
+// as many as the device runs side by side, fewer if there are not LEAST_TILES tiles for each.
+Plan plan_of(int n_seqs, int max_nodes, int max_kv_len, int n_heads, int n_kv, bool tensor) {
   Plan p;
-  const int group = n_heads / n_kv;
-  const long rows = (long)max_nodes * group;
-  p.wide_rows = rows > 16;
-  const int most = p.wide_rows ? 64 : 16;
-  p.rows_block = most;
-  const long units = (long)n_seqs * n_kv * ((rows + most - 1) / most), tiles = (max_kv_len + TILE - 1) / TILE;
+  const long rows = (long)max_nodes * (n_heads / n_kv);
+  p.rows_block = tensor ? (rows > 128 ? 256 : 128) : (rows > 16 ? 64 : 16);
+  const long units = (long)n_seqs * n_kv * ((rows + p.rows_block - 1) / p.rows_block), tiles = (max_kv_len + TILE - 1) / TILE;
   p.least = LEAST_TILES;
   const long wanted = units * ((tiles + p.least - 1) / p.least);
-  const long cap = 2L * gi::sm_count();
+  const long cap = (p.rows_block == 256 ? 1L : 2L) * gi::sm_count();
   p.blocks = (int)(wanted < cap ? (wanted > 1 ? wanted : 1) : cap);
   p.many_parts = p.blocks > 16 * units;
   return p;
 }
+
+long scratch_of(const Plan& p, int n_seqs, int hd) { return 8L * ((n_seqs + 2) / 2 * 2) + 2L * p.blocks * p.rows_block * (hd + 2) * 4; }
 
 template <typename T, int R, int DCH>
 int launch_tree(const Shape& sh, const Plan& p, T* out, long ldo, const T* q, long ldq, const T* k, const T* v, int cache_pages, int hd, float scale,
@@ -323,8 +322,10 @@ int launch_tree_dims(const Shape& sh, const Plan& p, T* out, long ldo, const T* 
 
 extern "C" long gi_attn_tree_scratch(int n_seqs, int max_nodes, int max_kv_len, int n_heads, int n_kv, int hd, int dtype) {
   if (n_seqs <= 0 || max_nodes <= 0 || max_kv_len <= 0 || n_kv <= 0 || n_heads < n_kv || hd <= 0) return 0;
-  const Plan p = plan_of(n_seqs, max_nodes, max_kv_len, n_heads, n_kv);
-  return 8L * (n_seqs + 2) + 2L * p.blocks * p.rows_block * (hd + 2) * 4;
+  const long plain = scratch_of(plan_of(n_seqs, max_nodes, max_kv_len, n_heads, n_kv, false), n_seqs, hd);
+  if (dtype != GI_BF16 || (hd != 64 && hd != 128)) return plain;
+  const long tensor = scratch_of(plan_of(n_seqs, max_nodes, max_kv_len, n_heads, n_kv, true), n_seqs, hd);
+  return tensor > plain ? tensor : plain;
 }
 
 extern "C" int gi_attn_tree(void* out, long ldo, const void* q, long ldq, int dtype, const void* kcache, const void* vcache, int cache_pages,
@@ -338,7 +339,10 @@ extern "C" int gi_attn_tree(void* out, long ldo, const void* q, long ldq, int dt
   if (words < (max_nodes + 31) / 32) return gi::fail(GI_ERR_ARG, "tree attention: %d words of mask bits cannot hold %d nodes", words, max_nodes);
   if (n_seqs > MAX_SEQS) return gi::fail(GI_ERR_UNSUPPORTED, "tree attention: more than %d sequences in one launch", MAX_SEQS);
   if (cache_pages < 1 || max_pages < 1 || max_kv_len < 1) return gi::fail(GI_ERR_ARG, "tree attention: %d pages, %d in a table's row, %d positions", cache_pages, max_pages, max_kv_len);
-  const Plan p = plan_of(n_seqs, max_nodes, max_kv_len, n_heads, n_kv);
+  // tensor cores: 16-bit rows and pages that TMA and 16-byte accesses can take, row coordinates of 32 bits
+  const bool tensor = dtype == GI_BF16 && (hd == 64 || hd == 128) && ldq % 8 == 0 && ldo % 8 == 0 && (((uintptr_t)q | (uintptr_t)kcache | (uintptr_t)vcache | (uintptr_t)out) & 15) == 0 &&
+                      (long)cache_pages * n_kv * TILE <= 0x7fffffffL;
+  const Plan p = plan_of(n_seqs, max_nodes, max_kv_len, n_heads, n_kv, tensor);
   if (scratch_bytes < gi_attn_tree_scratch(n_seqs, max_nodes, max_kv_len, n_heads, n_kv, hd, dtype) || ((uintptr_t)scratch & 15))
     return gi::fail(GI_ERR_ARG, "tree attention: the scratch memory is too small or not aligned");
   Shape sh = {cu_seqlens, seq_slots, seq_pos0, block_table, masks, words, max_pages, n_seqs, n_heads, n_kv, p.rows_block, max_nodes};
@@ -347,7 +351,9 @@ extern "C" int gi_attn_tree(void* out, long ldo, const void* q, long ldq, int dt
   float* part_ml = part_o + 2L * p.blocks * p.rows_block * hd;
   cudaStream_t s = (cudaStream_t)stream;
   int rc = GI_OK;
-  if (p.wide_rows)
+  if (tensor)
+    rc = launch_t5(sh, p.blocks, out, ldo, q, ldq, kcache, vcache, cache_pages, hd, scale, p.least, part_o, part_ml, prefix_out, s);
+  else if (p.rows_block == 64)
     GI_DISPATCH_DTYPE(dtype, T, rc = (launch_tree_dims<T, 64>(sh, p, (T*)out, ldo, (const T*)q, ldq, (const T*)kcache, (const T*)vcache, cache_pages, hd, scale, part_o, part_ml, prefix_out, s)));
   else
     GI_DISPATCH_DTYPE(dtype, T, rc = (launch_tree_dims<T, 16>(sh, p, (T*)out, ldo, (const T*)q, ldq, (const T*)kcache, (const T*)vcache, cache_pages, hd, scale, part_o, part_ml, prefix_out, s)));
@@ -355,6 +361,6 @@ extern "C" int gi_attn_tree(void* out, long ldo, const void* q, long ldq, int dt
   const int rows = max_nodes * (n_heads / n_kv);
   const dim3 join(p.many_parts ? rows : (rows + 7) / 8, n_kv, n_seqs);
   GI_DISPATCH_DTYPE(dtype, T, rc = gi::check(gi::launch(p.many_parts ? attn_tree_join_kernel<T, true> : attn_tree_join_kernel<T, false>, join, dim3(THREADS), 0, s, sh,
-                                                        (T*)out, ldo, hd, p.blocks, p.least, 0, part_o, part_ml, prefix_out), "tree attention (join)"));
+                                                        (T*)out, ldo, hd, p.blocks, p.least, tensor ? 1 : 0, part_o, part_ml, prefix_out), "tree attention (join)"));
   return rc;
 }

@@ -110,5 +110,9 @@ __device__ __forceinline__ int page_of(const Shape& s, int slot, int tile, int c
   return page >= 0 && page < cache_pages ? page : 0;
 }
 
+// The tensor-core form (attention_tree_t5.cu): rows_block 128 or 256, one or two row tiles a block.
+int launch_t5(const Shape& sh, int blocks, void* out, long ldo, const void* q, long ldq, const void* k, const void* v, int cache_pages, int hd,
+              float scale, int least, float* part_o, float* part_ml, long* part_prefix, cudaStream_t s);
+
 }  // namespace tree
 }  // namespace gi

@@ -160,6 +160,7 @@ def _bind():
         "gi_copy_pages": [P, P, P, P, P, I, P, P, P, I, P],
         "gi_attn_tree": [P, L, P, L, I, P, P, I, P, I, P, P, P, P, I, I, I, I, I, I, I, F, P, L, P],
         "gi_attn_tree_scratch": [I, I, I, I, I, I, I],
+        "gi_attn_tree_status": [P],
         "gi_tree_commit": [P, P, P, P, P, P, P, P, P, I, I, P, P, P, P, P, I, P, I, P],
         "gi_attn_decode_generic_ex3": [P, L, P, P, P, L, I, P, P, P, I, P, P, I, I, I, I, F, I, I, I, I, F, P, I, L, I, P],
     }
@@ -879,7 +880,7 @@ def check_status() -> None:
     clears the kernels' status words; synchronises the device."""
     bad = []
     for name, fn in (("prompt product", gemm_tc_status), ("decode product", gemm_stream_status),
-                     ("prompt attention", attn_prefill_t5_status)):
+                     ("prompt attention", attn_prefill_t5_status), ("tree attention", attn_tree_status)):
         code = fn()
         if code:
             bad.append(f"{name} (wait {code})")
@@ -1060,6 +1061,14 @@ def attn_prefill_t5_status() -> int:
     lib = _bind()
     status = ctypes.c_int(0)
     _check(lib, lib.gi_attn_prefill_t5_status(ctypes.byref(status)), 0)
+    return status.value
+
+
+def attn_tree_status() -> int:
+    """0 if every wait inside the tensor-core tree attention was met since the last call; synchronises the device."""
+    lib = _bind()
+    status = ctypes.c_int(0)
+    _check(lib, lib.gi_attn_tree_status(ctypes.byref(status)), 0)
     return status.value
 
 
