@@ -699,7 +699,7 @@ int gi_copy_pages(void* const* tensors, const int* layers, const int* pages, con
 // max_kv_len that is too small costs time only.  hd 1 to 256, n_seqs at most 1024.  scratch: gi_attn_tree_scratch bytes, 16-byte
 // aligned.  Keys and values of nodes that nobody sees, and what lies behind the last node, may hold anything.
 long gi_attn_tree_scratch(int n_seqs, int max_nodes, int max_kv_len, int n_heads, int n_kv, int hd, int dtype);
-int gi_attn_tree(void* out, long ldo, const void* q, long ldq, int dtype, const void* kcache, const void* vcache, int cache_pages,
+int gi_attn_tree(void* out, long ldo, const void* q, long ldq, long q_rows, int dtype, const void* kcache, const void* vcache, int cache_pages,
                  const int* block_table, int max_pages, const int* cu_seqlens, const int* seq_slots, const int* seq_pos0, const int* masks,
                  int words, int n_seqs, int max_nodes, int max_kv_len, int n_heads, int n_kv, int hd, float scale, void* scratch,
                  long scratch_bytes, void* stream);

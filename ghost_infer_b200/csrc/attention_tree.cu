@@ -20,11 +20,12 @@ namespace {
 using namespace gi::tree;
 
 constexpr int THREADS = 256;
+constexpr int TILE = 64;
 
 template <typename T, int R, int DCH>
 __global__ void __launch_bounds__(THREADS)
-attn_tree_kernel(const Shape sh, T* __restrict__ out, long ldo, const T* q, long ldq, const T* kcache, const T* vcache, int cache_pages, int hd, float scale,
-                 int least, float* __restrict__ part_o, float* __restrict__ part_ml, long* __restrict__ part_prefix, int vec) {
+attn_tree_kernel(const Shape sh, T* __restrict__ out, long ldo, const T* q, long ldq, const T* kcache, const T* vcache, int hd, float scale,
+                 float4* __restrict__ part_o, float2* __restrict__ part_ml, int* __restrict__ part_prefix, int vec) {
   constexpr int RT = R / 16;                       // rows a thread works on: ty + 16 i
   extern __shared__ __align__(16) float smem[];
   const int hp = (hd + 3) / 4 * 4, ld = hp + 4;    // rows padded: 16 rows' four-number reads fall into different banks
@@ -32,20 +33,20 @@ attn_tree_kernel(const Shape sh, T* __restrict__ out, long ldo, const T* q, long
   float* Ks = Qs + R * ld;                         // [64][ld]
   float* Vs = Ks + TILE * ld;                      // [64][ld]
   float* Ps = Vs + TILE * ld;                      // [R][68]
-  __shared__ long s_pre[MAX_SEQS + 1];
+  __shared__ int s_pre[MAX_SEQS + 1];
   const int tid = threadIdx.x, ty = tid >> 4, tx = tid & 15;
   gi::pdl_prologue();
   if (tid < 32) prefix(sh, s_pre);
   __syncthreads();
-  const long total = s_pre[sh.n_seqs], per = per_block(total, gridDim.x, least);
+  const int total = s_pre[sh.n_seqs], per = per_range(sh, total, gridDim.x);
   if (blockIdx.x == 0)
     for (int i = tid; i <= sh.n_seqs; i += THREADS) part_prefix[i] = s_pre[i];
-  const long lo = (long)blockIdx.x * per, hi = min(total, lo + per);
+  const int lo = (int)min((long)total, (long)blockIdx.x * per), hi = min(total, lo + per);
   const int group = sh.n_heads / sh.n_kv;
 
-  for (long at = lo; at < hi;) {
+  for (int at = lo; at < hi;) {
     const Unit u = unit_at(sh, s_pre, at);
-    const int t_begin = (int)(at - u.first), t_end = (int)min((long)u.tiles, hi - u.first);
+    const int t_begin = at - u.first, t_end = min(u.tiles, hi - u.first);
     const int tok0 = sh.cu_seqlens[u.b], len = u.pos0 + u.n;
     const int rows_here = min(sh.rows_block, u.n * group - u.row0);
     __syncthreads();
@@ -62,7 +63,7 @@ attn_tree_kernel(const Shape sh, T* __restrict__ out, long ldo, const T* q, long
     }
     for (int t = t_begin; t < t_end; ++t) {
       const int kt = t * TILE;
-      const int page = page_of(sh, u.slot, t, cache_pages);
+      const int page = page_of(sh, u.slot, t);
       const size_t base = ((size_t)page * sh.n_kv + u.kvh) * TILE * hd;
       __syncthreads();
       if (vec) {
@@ -189,111 +190,137 @@ attn_tree_kernel(const Shape sh, T* __restrict__ out, long ldo, const T* q, long
       T* dst = out + (size_t)(tok0 + row / group) * ldo + (size_t)(u.kvh * group + row % group) * hd;
       const float inv = l[i] == 0.f ? 0.f : 1.0f / l[i];
 #pragma unroll
-      for (int c = 0; c < DCH * 4; ++c) {
-        const int d = (c / 4) * 64 + tx * 4 + (c & 3);
-        if (d >= hd) continue;
-        if (whole) gi::stf(dst + d, acc[i][c] * inv);
-        else part_o[(slot2 * sh.rows_block + r) * hd + d] = acc[i][c];
+      for (int c = 0; c < DCH; ++c) {
+        const int d = c * 64 + tx * 4;
+        if (whole) {
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            if (d + e < hd) gi::stf(dst + d + e, acc[i][c * 4 + e] * inv);
+        } else if (d < hd) {
+          part_o[part_at(sh, slot2, hp / 4, d / 4, r)] = make_float4(acc[i][c * 4], acc[i][c * 4 + 1], acc[i][c * 4 + 2], acc[i][c * 4 + 3]);
+        }
       }
-      if (!whole && tx == 0) {
-        part_ml[(slot2 * sh.rows_block + r) * 2] = m[i];
-        part_ml[(slot2 * sh.rows_block + r) * 2 + 1] = l[i];
-      }
+      if (!whole && tx == 0) part_ml[slot2 * sh.rows_block + r] = make_float2(m[i], l[i]);
     }
     at = u.first + t_end;
   }
 }
 
-// Joins the parts of the units that several blocks hold; maxima are in units of ln (base 1) or of powers of two (base2).  A warp
-// takes a row's parts, or, where a row may have many, all warps of a block do and meet in shared memory.
-template <typename T, bool SHARED_ROWS>
+// Joins the parts of the units that several blocks hold; maxima are in units of ln, or of powers of two (base2).  A block takes 32
+// query rows of a kv head, one to a lane.  Its warps share out the head's numbers, or (MANY: a unit may lie on dozens of blocks)
+// the parts, for 16 of the head's numbers a block, and meet in shared memory.
+template <typename T, bool MANY>
 __global__ void __launch_bounds__(THREADS)
-attn_tree_join_kernel(const Shape sh, T* __restrict__ out, long ldo, int hd, int blocks, int least, int base2, const float* part_o, const float* part_ml,
-                      const long* part_prefix) {
-  constexpr int WARPS = THREADS / 32, NUMBERS = 8;         // numbers of a head per lane: head sizes up to 256
-  __shared__ float s_acc[SHARED_ROWS ? WARPS : 1][256];
-  __shared__ float s_l[WARPS];
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+attn_tree_join_kernel(const Shape sh, T* __restrict__ out, long ldo, int hd, int ranges, int base2, const float4* part_o, const float2* part_ml,
+                      const int* part_prefix) {
+  constexpr int WARPS = THREADS / 32, FOURS = 4;           // pieces of four numbers that a thread holds at a time
+  __shared__ float s_acc[MANY ? WARPS : 1][FOURS * 4 + 1][33];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, fours = (hd + 3) / 4;
   gi::pdl_prologue();
-  const int b = blockIdx.z, kvh = blockIdx.y, group = sh.n_heads / sh.n_kv;
-  const int row = SHARED_ROWS ? blockIdx.x : blockIdx.x * WARPS + warp;
+  const int b = blockIdx.z, group = sh.n_heads / sh.n_kv;
+  const int cuts = MANY ? (fours + FOURS - 1) / FOURS : 1;
+  const int kvh = blockIdx.y, row = blockIdx.x / cuts * 32 + lane, cut = blockIdx.x % cuts;
   const int n = nodes_of(sh, b);
-  if (row >= n * group) return;                            // (a block's rows: the same for all of a block that meets)
-  const long total = part_prefix[sh.n_seqs], per = per_block(total, blocks, least);
-  const int tiles = (pos0_of(sh, b) + n + TILE - 1) / TILE;
-  const long first = part_prefix[b] + ((long)(row / sh.rows_block) * sh.n_kv + kvh) * tiles;
-  const int c0 = (int)(first / per), c1 = (int)((first + tiles - 1) / per);
-  if (c0 == c1) return;                                    // one block had it all
+  const int per = per_range(sh, part_prefix[sh.n_seqs], ranges);
+  const int tiles = tiles_of(sh, pos0_of(sh, b), n), row_block = row / sh.rows_block;
+  const int first = part_prefix[b] + (row_block / sh.split * sh.n_kv + kvh) * tiles;
+  int c0 = 0, c1 = 0;
+  if (row < n * group) c0 = first / per, c1 = (first + tiles - 1) / per;
+  const bool live = c0 != c1;                              // (one block had it all, or there is no such row)
+  if (__all_sync(0xffffffffu, !live)) return;              // (every warp of the block has the same rows)
   const int r = row % sh.rows_block;
-  auto slot_of = [&](int c) { return (2 * (size_t)c + (c == c0 ? 1 : 0)) * sh.rows_block + r; };
-  float m = -INFINITY, l = 0.f, acc[NUMBERS];
-#pragma unroll
-  for (int i = 0; i < NUMBERS; ++i) acc[i] = 0.f;
-  for (int c = c0 + lane; c <= c1; c += 32) m = fmaxf(m, part_ml[slot_of(c) * 2]);
-  m = gi::warp_max(m);
-  const float ref = m == -INFINITY ? 0.f : m;
-#pragma unroll 2
-  for (int c = c0 + (SHARED_ROWS ? warp : 0); c <= c1; c += SHARED_ROWS ? WARPS : 1) {
-    const size_t s = slot_of(c);
-    const float pm = part_ml[s * 2], pl = part_ml[s * 2 + 1];
-    const float w = base2 ? exp2f(pm - ref) : expf(pm - ref);
-    l += w * pl;
-#pragma unroll
-    for (int i = 0; i < NUMBERS; ++i)
-      if (lane + 32 * i < hd) {
-        const float o = part_o[s * hd + lane + 32 * i];
-        if (w != 0.f) acc[i] = fmaf(w, o, acc[i]);
-      }
+  auto slot_of = [&](int c) { return 2 * ((size_t)c * sh.split + row_block % sh.split) + (c == c0 ? 1 : 0); };
+  float ref = -INFINITY;
+  if (live) {
+#pragma unroll 4
+    for (int c = c0; c <= c1; ++c) ref = fmaxf(ref, part_ml[slot_of(c) * sh.rows_block + r].x);
   }
+  if (ref == -INFINITY) ref = 0.f;
   T* dst = out + (size_t)(sh.cu_seqlens[b] + row / group) * ldo + (size_t)(kvh * group + row % group) * hd;
-  if (SHARED_ROWS) {
+  for (int four0 = MANY ? cut * FOURS : warp * FOURS; four0 < fours; four0 += MANY ? fours : WARPS * FOURS) {
+    float l = 0.f, acc[FOURS][4];
 #pragma unroll
-    for (int i = 0; i < NUMBERS; ++i) s_acc[warp][lane + 32 * i] = acc[i];
-    if (lane == 0) s_l[warp] = l;
-    __syncthreads();
-    l = 0.f;
-    for (int w = 0; w < WARPS; ++w) l += s_l[w];
-    const float inv = l == 0.f ? 0.f : 1.0f / l;
-    for (int d = threadIdx.x; d < hd; d += THREADS) {
-      float o = 0.f;
-      for (int w = 0; w < WARPS; ++w) o += s_acc[w][d];
-      gi::stf(dst + d, o * inv);
+    for (int k = 0; k < FOURS; ++k)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) acc[k][e] = 0.f;
+    if (live) {
+#pragma unroll 2
+      for (int c = c0 + (MANY ? warp : 0); c <= c1; c += MANY ? WARPS : 1) {
+        const size_t s = slot_of(c);
+        const float2 ml = part_ml[s * sh.rows_block + r];
+        float4 o[FOURS];
+#pragma unroll
+        for (int k = 0; k < FOURS; ++k)
+          if (four0 + k < fours) o[k] = part_o[part_at(sh, s, fours, four0 + k, r)];
+        const float w = base2 ? exp2f(ml.x - ref) : expf(ml.x - ref);
+        l += w * ml.y;
+#pragma unroll
+        for (int k = 0; k < FOURS; ++k)
+          if (four0 + k < fours && w != 0.f) {
+            acc[k][0] = fmaf(w, o[k].x, acc[k][0]);
+            acc[k][1] = fmaf(w, o[k].y, acc[k][1]);
+            acc[k][2] = fmaf(w, o[k].z, acc[k][2]);
+            acc[k][3] = fmaf(w, o[k].w, acc[k][3]);
+          }
+      }
     }
-    return;
-  }
-  const float inv = l == 0.f ? 0.f : 1.0f / l;
+    if (MANY) {
 #pragma unroll
-  for (int i = 0; i < NUMBERS; ++i)
-    if (lane + 32 * i < hd) gi::stf(dst + lane + 32 * i, acc[i] * inv);
+      for (int k = 0; k < FOURS; ++k)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) s_acc[warp][k * 4 + e][lane] = acc[k][e];
+      s_acc[warp][FOURS * 4][lane] = l;
+      __syncthreads();
+      if (warp != 0) return;
+#pragma unroll
+      for (int k = 0; k < FOURS; ++k)
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          for (int w = 1; w < WARPS; ++w) acc[k][e] += s_acc[w][k * 4 + e][lane];
+      for (int w = 1; w < WARPS; ++w) l += s_acc[w][FOURS * 4][lane];
+    }
+    const float inv = l == 0.f ? 0.f : 1.0f / l;
+    if (live) {
+#pragma unroll
+      for (int k = 0; k < FOURS; ++k)
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          if ((four0 + k) * 4 + e < hd) gi::stf(dst + (four0 + k) * 4 + e, acc[k][e] * inv);
+    }
+  }
 }
 
 struct Plan {
-  int blocks, least, rows_block;
+  int ranges, split, rows_block, tile, least;
   bool many_parts;      // a unit may lie on more blocks than one warp should join
 };
 
-constexpr int LEAST_TILES = 2;
-
-// The query rows of a block: 16 or 64 on CUDA cores, 128 or 256 on tensor cores, the smaller where it holds a tree's rows; blocks:
-// as many as the device runs side by side, fewer if there are not LEAST_TILES tiles for each.
+// The query rows of a block: 16 or 64 on CUDA cores, the smaller where it takes a tree's rows; on tensor cores as many whole nodes as
+// 128 lanes hold, and up to 8 row blocks of a unit side by side.  Blocks: as many as the device runs at a time, fewer if
+// there are not `least` tiles for each.
 Plan plan_of(int n_seqs, int max_nodes, int max_kv_len, int n_heads, int n_kv, bool tensor) {
   Plan p;
-  const long rows = (long)max_nodes * (n_heads / n_kv);
-  p.rows_block = tensor ? (rows > 128 ? 256 : 128) : (rows > 16 ? 64 : 16);
-  const long units = (long)n_seqs * n_kv * ((rows + p.rows_block - 1) / p.rows_block), tiles = (max_kv_len + TILE - 1) / TILE;
-  p.least = LEAST_TILES;
+  const int group = n_heads / n_kv;
+  const long rows = (long)max_nodes * group;
+  p.rows_block = tensor ? 128 / group * group : (rows > 16 ? 64 : 16);
+  p.tile = tensor ? 128 : TILE;
+  p.least = tensor ? 1 : 2;
+  const long blocks = (rows + p.rows_block - 1) / p.rows_block, rounds = tensor ? (blocks + 7) / 8 : blocks;
+  p.split = (int)((blocks + rounds - 1) / rounds);
+  const long units = (long)n_seqs * n_kv * rounds, tiles = (max_kv_len + p.tile - 1) / p.tile;
   const long wanted = units * ((tiles + p.least - 1) / p.least);
-  const long cap = (p.rows_block == 256 ? 1L : 2L) * gi::sm_count();
-  p.blocks = (int)(wanted < cap ? (wanted > 1 ? wanted : 1) : cap);
-  p.many_parts = p.blocks > 16 * units;
+  const long cap = (tensor ? 1L : 2L) * gi::sm_count() / p.split;
+  p.ranges = (int)(wanted < cap ? wanted : cap);
+  if (p.ranges < 1) p.ranges = 1;
+  p.many_parts = p.ranges > 16 * units;
   return p;
 }
 
-long scratch_of(const Plan& p, int n_seqs, int hd) { return 8L * ((n_seqs + 2) / 2 * 2) + 2L * p.blocks * p.rows_block * (hd + 2) * 4; }
+long scratch_of(const Plan& p, int n_seqs, int hd) { return 4L * ((n_seqs + 4) / 4 * 4) + 2L * p.ranges * p.split * p.rows_block * ((hd + 3) / 4 * 4 + 2) * 4; }
 
 template <typename T, int R, int DCH>
-int launch_tree(const Shape& sh, const Plan& p, T* out, long ldo, const T* q, long ldq, const T* k, const T* v, int cache_pages, int hd, float scale,
-                float* part_o, float* part_ml, long* part_prefix, cudaStream_t s) {
+int launch_tree(const Shape& sh, const Plan& p, T* out, long ldo, const T* q, long ldq, const T* k, const T* v, int hd, float scale,
+                float4* part_o, float2* part_ml, int* part_prefix, cudaStream_t s) {
   const int hp = (hd + 3) / 4 * 4;
   const size_t smem = ((size_t)(R + 2 * TILE) * (hp + 4) + (size_t)R * 68) * sizeof(float);
   auto kern = attn_tree_kernel<T, R, DCH>;
@@ -306,16 +333,15 @@ int launch_tree(const Shape& sh, const Plan& p, T* out, long ldo, const T* q, lo
     if (dev >= 0) configured[dev] = true;
   }
   const int vec = hd % 4 == 0 && ((uintptr_t)k % (4 * sizeof(T))) == 0 && ((uintptr_t)v % (4 * sizeof(T))) == 0;
-  return gi::check(gi::launch(kern, dim3(p.blocks), dim3(THREADS), smem, s, sh, out, ldo, q, ldq, k, v, cache_pages, hd, scale, p.least, part_o, part_ml,
-                              part_prefix, vec), "tree attention");
+  return gi::check(gi::launch(kern, dim3(p.ranges), dim3(THREADS), smem, s, sh, out, ldo, q, ldq, k, v, hd, scale, part_o, part_ml, part_prefix, vec), "tree attention");
 }
 
 template <typename T, int R>
-int launch_tree_dims(const Shape& sh, const Plan& p, T* out, long ldo, const T* q, long ldq, const T* k, const T* v, int cache_pages, int hd, float scale,
-                     float* part_o, float* part_ml, long* part_prefix, cudaStream_t s) {
-  if (hd <= 64) return launch_tree<T, R, 1>(sh, p, out, ldo, q, ldq, k, v, cache_pages, hd, scale, part_o, part_ml, part_prefix, s);
-  if (hd <= 128) return launch_tree<T, R, 2>(sh, p, out, ldo, q, ldq, k, v, cache_pages, hd, scale, part_o, part_ml, part_prefix, s);
-  return launch_tree<T, R, 4>(sh, p, out, ldo, q, ldq, k, v, cache_pages, hd, scale, part_o, part_ml, part_prefix, s);
+int launch_tree_dims(const Shape& sh, const Plan& p, T* out, long ldo, const T* q, long ldq, const T* k, const T* v, int hd, float scale,
+                     float4* part_o, float2* part_ml, int* part_prefix, cudaStream_t s) {
+  if (hd <= 64) return launch_tree<T, R, 1>(sh, p, out, ldo, q, ldq, k, v, hd, scale, part_o, part_ml, part_prefix, s);
+  if (hd <= 128) return launch_tree<T, R, 2>(sh, p, out, ldo, q, ldq, k, v, hd, scale, part_o, part_ml, part_prefix, s);
+  return launch_tree<T, R, 4>(sh, p, out, ldo, q, ldq, k, v, hd, scale, part_o, part_ml, part_prefix, s);
 }
 
 }  // namespace
@@ -323,12 +349,12 @@ int launch_tree_dims(const Shape& sh, const Plan& p, T* out, long ldo, const T* 
 extern "C" long gi_attn_tree_scratch(int n_seqs, int max_nodes, int max_kv_len, int n_heads, int n_kv, int hd, int dtype) {
   if (n_seqs <= 0 || max_nodes <= 0 || max_kv_len <= 0 || n_kv <= 0 || n_heads < n_kv || hd <= 0) return 0;
   const long plain = scratch_of(plan_of(n_seqs, max_nodes, max_kv_len, n_heads, n_kv, false), n_seqs, hd);
-  if (dtype != GI_BF16 || (hd != 64 && hd != 128)) return plain;
+  if (dtype != GI_BF16 || (hd != 64 && hd != 128) || n_heads / n_kv > 128) return plain;
   const long tensor = scratch_of(plan_of(n_seqs, max_nodes, max_kv_len, n_heads, n_kv, true), n_seqs, hd);
   return tensor > plain ? tensor : plain;
 }
 
-extern "C" int gi_attn_tree(void* out, long ldo, const void* q, long ldq, int dtype, const void* kcache, const void* vcache, int cache_pages,
+extern "C" int gi_attn_tree(void* out, long ldo, const void* q, long ldq, long q_rows, int dtype, const void* kcache, const void* vcache, int cache_pages,
                             const int* block_table, int max_pages, const int* cu_seqlens, const int* seq_slots, const int* seq_pos0, const int* masks,
                             int words, int n_seqs, int max_nodes, int max_kv_len, int n_heads, int n_kv, int hd, float scale, void* scratch,
                             long scratch_bytes, void* stream) {
@@ -340,27 +366,30 @@ extern "C" int gi_attn_tree(void* out, long ldo, const void* q, long ldq, int dt
   if (n_seqs > MAX_SEQS) return gi::fail(GI_ERR_UNSUPPORTED, "tree attention: more than %d sequences in one launch", MAX_SEQS);
   if (cache_pages < 1 || max_pages < 1 || max_kv_len < 1) return gi::fail(GI_ERR_ARG, "tree attention: %d pages, %d in a table's row, %d positions", cache_pages, max_pages, max_kv_len);
   // tensor cores: 16-bit rows and pages that TMA and 16-byte accesses can take, row coordinates of 32 bits
-  const bool tensor = dtype == GI_BF16 && (hd == 64 || hd == 128) && ldq % 8 == 0 && ldo % 8 == 0 && (((uintptr_t)q | (uintptr_t)kcache | (uintptr_t)vcache | (uintptr_t)out) & 15) == 0 &&
-                      (long)cache_pages * n_kv * TILE <= 0x7fffffffL;
+  const bool tensor = dtype == GI_BF16 && (hd == 64 || hd == 128) && n_heads / n_kv <= 128 && q_rows <= 0x7fffffffL && ldq % 8 == 0 && ldo % 8 == 0 && (((uintptr_t)q | (uintptr_t)kcache | (uintptr_t)vcache | (uintptr_t)out) & 15) == 0 &&
+                      (long)cache_pages * n_kv * PAGE_TOKENS <= 0x7fffffffL;
   const Plan p = plan_of(n_seqs, max_nodes, max_kv_len, n_heads, n_kv, tensor);
   if (scratch_bytes < gi_attn_tree_scratch(n_seqs, max_nodes, max_kv_len, n_heads, n_kv, hd, dtype) || ((uintptr_t)scratch & 15))
     return gi::fail(GI_ERR_ARG, "tree attention: the scratch memory is too small or not aligned");
-  Shape sh = {cu_seqlens, seq_slots, seq_pos0, block_table, masks, words, max_pages, n_seqs, n_heads, n_kv, p.rows_block, max_nodes};
-  long* prefix_out = (long*)scratch;
-  float* part_o = (float*)(prefix_out + (n_seqs + 2) / 2 * 2);
-  float* part_ml = part_o + 2L * p.blocks * p.rows_block * hd;
+  // the list of tiles is counted in 32 bits
+  const long most = (long)n_seqs * n_kv * (((long)max_nodes * (n_heads / n_kv) + p.rows_block - 1) / p.rows_block) * (((long)max_pages * PAGE_TOKENS + max_nodes) / p.tile + 1);
+  if (most > 0x3fffffffL || max_pages > 0x7fffffff / PAGE_TOKENS - MAX_NODES) return gi::fail(GI_ERR_UNSUPPORTED, "tree attention: %d sequences of up to %d pages are more than one launch takes", n_seqs, max_pages);
+  const Shape sh = {cu_seqlens, seq_slots, seq_pos0, block_table, masks, words, max_pages, n_seqs, n_heads, n_kv, max_nodes, cache_pages, p.rows_block, p.split, p.tile, p.least};
+  int* prefix_out = (int*)scratch;
+  float4* part_o = (float4*)(prefix_out + (n_seqs + 4) / 4 * 4);
+  float2* part_ml = (float2*)(part_o + 2L * p.ranges * p.split * p.rows_block * ((hd + 3) / 4));
   cudaStream_t s = (cudaStream_t)stream;
   int rc = GI_OK;
   if (tensor)
-    rc = launch_t5(sh, p.blocks, out, ldo, q, ldq, kcache, vcache, cache_pages, hd, scale, p.least, part_o, part_ml, prefix_out, s);
+    rc = launch_t5(sh, p.ranges * p.split, out, ldo, q, ldq, q_rows, kcache, vcache, hd, scale, part_o, part_ml, prefix_out, s);
   else if (p.rows_block == 64)
-    GI_DISPATCH_DTYPE(dtype, T, rc = (launch_tree_dims<T, 64>(sh, p, (T*)out, ldo, (const T*)q, ldq, (const T*)kcache, (const T*)vcache, cache_pages, hd, scale, part_o, part_ml, prefix_out, s)));
+    GI_DISPATCH_DTYPE(dtype, T, rc = (launch_tree_dims<T, 64>(sh, p, (T*)out, ldo, (const T*)q, ldq, (const T*)kcache, (const T*)vcache, hd, scale, part_o, part_ml, prefix_out, s)));
   else
-    GI_DISPATCH_DTYPE(dtype, T, rc = (launch_tree_dims<T, 16>(sh, p, (T*)out, ldo, (const T*)q, ldq, (const T*)kcache, (const T*)vcache, cache_pages, hd, scale, part_o, part_ml, prefix_out, s)));
+    GI_DISPATCH_DTYPE(dtype, T, rc = (launch_tree_dims<T, 16>(sh, p, (T*)out, ldo, (const T*)q, ldq, (const T*)kcache, (const T*)vcache, hd, scale, part_o, part_ml, prefix_out, s)));
   if (rc != GI_OK) return rc;
   const int rows = max_nodes * (n_heads / n_kv);
-  const dim3 join(p.many_parts ? rows : (rows + 7) / 8, n_kv, n_seqs);
+  const dim3 join((unsigned)((rows + 31) / 32 * (p.many_parts ? (hd + 15) / 16 : 1)), n_kv, n_seqs);
   GI_DISPATCH_DTYPE(dtype, T, rc = gi::check(gi::launch(p.many_parts ? attn_tree_join_kernel<T, true> : attn_tree_join_kernel<T, false>, join, dim3(THREADS), 0, s, sh,
-                                                        (T*)out, ldo, hd, p.blocks, p.least, tensor ? 1 : 0, part_o, part_ml, prefix_out), "tree attention (join)"));
+                                                        (T*)out, ldo, hd, p.ranges, tensor ? 1 : 0, part_o, part_ml, prefix_out), "tree attention (join)"));
   return rc;
 }

@@ -422,6 +422,19 @@ int gi::tensor_map_2d_ex(CUtensorMap* out, const void* base, long rows, long col
   return GI_OK;
 }
 
+int gi::tensor_map_3d(CUtensorMap* out, const void* base, long rows, long heads, long cols, long row_ld, long head_ld, int box_cols, int box_heads, int box_rows) {
+  EncodeTiled enc = encoder();
+  if (!enc) return gi::fail(GI_ERR_CUDA, "tensor map: the driver does not export cuTensorMapEncodeTiled");
+  const cuuint64_t dims[3] = {(cuuint64_t)cols, (cuuint64_t)heads, (cuuint64_t)rows};
+  const cuuint64_t strides[2] = {(cuuint64_t)head_ld * 2, (cuuint64_t)row_ld * 2};
+  const cuuint32_t box[3] = {(cuuint32_t)box_cols, (cuuint32_t)box_heads, (cuuint32_t)box_rows};
+  const cuuint32_t estr[3] = {1, 1, 1};
+  CUresult r = enc(out, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, const_cast<void*>(base), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                   CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS) return gi::fail(GI_ERR_CUDA, "tensor map of three dimensions: cuTensorMapEncodeTiled failed with %d", (int)r);
+  return GI_OK;
+}
+
 int gi::tensor_map_2d(CUtensorMap* out, const void* base, int rows, int cols, long ld, int box_rows) {
   return gi::tensor_map_2d_ex(out, base, rows, cols, ld, GI_BF16, BK, box_rows);
 }

@@ -88,5 +88,8 @@ __device__ __forceinline__ void mbar_arrive(uint32_t bar) {
 int tensor_map_2d(CUtensorMap* out, const void* base, int rows, int cols, long ld, int box_rows);
 // The general form: `elem` is GI_F32 or GI_BF16, the box is box_cols x box_rows elements (box_cols * element size = 128 bytes).
 int tensor_map_2d_ex(CUtensorMap* out, const void* base, long rows, long cols, long ld, int elem, int box_cols, int box_rows);
+// Rows of several heads as [rows][heads][cols] bfloat16 (strides row_ld, head_ld; 128-byte swizzle, zero fill outside): a box is
+// box_rows x box_heads rows of box_cols columns, a row's heads one below the other.
+int tensor_map_3d(CUtensorMap* out, const void* base, long rows, long heads, long cols, long row_ld, long head_ld, int box_cols, int box_heads, int box_rows);
 
 }  // namespace gi

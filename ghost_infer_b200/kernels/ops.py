@@ -158,7 +158,7 @@ def _bind():
         "gi_beam_select_scratch": [I, I, I],
         "gi_reorder_states": [P, P, I, I, P, P, I, I, I, P],
         "gi_copy_pages": [P, P, P, P, P, I, P, P, P, I, P],
-        "gi_attn_tree": [P, L, P, L, I, P, P, I, P, I, P, P, P, P, I, I, I, I, I, I, I, F, P, L, P],
+        "gi_attn_tree": [P, L, P, L, L, I, P, P, I, P, I, P, P, P, P, I, I, I, I, I, I, I, F, P, L, P],
         "gi_attn_tree_scratch": [I, I, I, I, I, I, I],
         "gi_attn_tree_status": [P],
         "gi_tree_commit": [P, P, P, P, P, P, P, P, P, I, I, P, P, P, P, P, I, P, I, P],
@@ -3019,7 +3019,7 @@ def attention_tree(q: torch.Tensor, kcache: torch.Tensor, vcache: torch.Tensor, 
     cu, ss, sp = _i32_of(cu_seqlens, n_seqs + 1, "cu_seqlens"), _i32_of(seq_slots, n_seqs, "slots"), _i32_of(seq_pos0, n_seqs, "start positions")
     nbytes = lib.gi_attn_tree_scratch(n_seqs, max_nodes, max_kv_len, n_heads, n_kv, head_dim, dt)
     scratch = torch.empty((max(nbytes, 16),), dtype=torch.uint8, device=q.device)
-    _check(lib, lib.gi_attn_tree(out.data_ptr(), ldo, q.data_ptr(), ldq, dt, kcache.data_ptr(), vcache.data_ptr(), kcache.shape[0],
+    _check(lib, lib.gi_attn_tree(out.data_ptr(), ldo, q.data_ptr(), ldq, q.shape[0], dt, kcache.data_ptr(), vcache.data_ptr(), kcache.shape[0],
                                  _i32(block_table, "block table"), block_table.shape[1], cu, ss, sp, masks.data_ptr(), masks.shape[1], n_seqs, max_nodes,
                                  max_kv_len, n_heads, n_kv, head_dim, float(scale), scratch.data_ptr(), nbytes, _stream()), 2 if n_seqs else 0)
     return out
