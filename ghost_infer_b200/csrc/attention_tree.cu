@@ -207,92 +207,94 @@ attn_tree_kernel(const Shape sh, T* __restrict__ out, long ldo, const T* q, long
 }
 
 // Joins the parts of the units that several blocks hold; maxima are in units of ln, or of powers of two (base2).  A block takes 32
-// query rows of a kv head, one to a lane.  Its warps share out the head's numbers, or (MANY: a unit may lie on dozens of blocks)
-// the parts, for 16 of the head's numbers a block, and meet in shared memory.
-template <typename T, bool MANY>
+// query rows of a kv head, one to a lane, and 16 of the head's numbers for each of WARPS / PARTS warps; PARTS warps share out a
+// row's parts.  A part's maximum, sum and values are asked for together and joined as they come (one trip to memory, not one
+// for the maxima and then one for the values); the warps meet in shared memory.
+template <typename T, int PARTS>
 __global__ void __launch_bounds__(THREADS)
 attn_tree_join_kernel(const Shape sh, T* __restrict__ out, long ldo, int hd, int ranges, int base2, const float4* part_o, const float2* part_ml,
                       const int* part_prefix) {
-  constexpr int WARPS = THREADS / 32, FOURS = 4;           // pieces of four numbers that a thread holds at a time
-  __shared__ float s_acc[MANY ? WARPS : 1][FOURS * 4 + 1][33];
+  constexpr int WARPS = THREADS / 32, CUTS = WARPS / PARTS, FOURS = 4;      // pieces of four numbers that a thread holds
+  __shared__ float s_acc[WARPS][FOURS * 4 + 2][33];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, fours = (hd + 3) / 4;
   gi::pdl_prologue();
   const int b = blockIdx.z, group = sh.n_heads / sh.n_kv;
-  const int cuts = MANY ? (fours + FOURS - 1) / FOURS : 1;
-  const int kvh = blockIdx.y, row = blockIdx.x / cuts * 32 + lane, cut = blockIdx.x % cuts;
-  const int n = nodes_of(sh, b);
-  const int per = per_range(sh, part_prefix[sh.n_seqs], ranges);
-  const int tiles = tiles_of(sh, pos0_of(sh, b), n), row_block = row / sh.rows_block;
-  const int first = part_prefix[b] + (row_block / sh.split * sh.n_kv + kvh) * tiles;
+  const int cuts = (fours + CUTS * FOURS - 1) / (CUTS * FOURS);             // blocks along a head's numbers
+  const int kvh = blockIdx.y, row = blockIdx.x / cuts * 32 + lane;
+  const int part_group = warp % PARTS, four0 = ((blockIdx.x % cuts) * CUTS + warp / PARTS) * FOURS;
+  const int total = part_prefix[sh.n_seqs], before = part_prefix[b], n = nodes_of(sh, b), pos0 = pos0_of(sh, b), tok0 = sh.cu_seqlens[b];
+  const int per = per_range(sh, total, ranges);
+  const int tiles = tiles_of(sh, pos0, n), row_block = row / sh.rows_block, r = row - row_block * sh.rows_block;
+  const int first = before + (row_block / sh.split * sh.n_kv + kvh) * tiles;
   int c0 = 0, c1 = 0;
   if (row < n * group) c0 = first / per, c1 = (first + tiles - 1) / per;
   const bool live = c0 != c1;                              // (one block had it all, or there is no such row)
   if (__all_sync(0xffffffffu, !live)) return;              // (every warp of the block has the same rows)
-  const int r = row % sh.rows_block;
-  auto slot_of = [&](int c) { return 2 * ((size_t)c * sh.split + row_block % sh.split) + (c == c0 ? 1 : 0); };
-  float ref = -INFINITY;
-  if (live) {
-#pragma unroll 4
-    for (int c = c0; c <= c1; ++c) ref = fmaxf(ref, part_ml[slot_of(c) * sh.rows_block + r].x);
-  }
-  if (ref == -INFINITY) ref = 0.f;
-  T* dst = out + (size_t)(sh.cu_seqlens[b] + row / group) * ldo + (size_t)(kvh * group + row % group) * hd;
-  for (int four0 = MANY ? cut * FOURS : warp * FOURS; four0 < fours; four0 += MANY ? fours : WARPS * FOURS) {
-    float l = 0.f, acc[FOURS][4];
+  float m = -INFINITY, l = 0.f, acc[FOURS][4];
 #pragma unroll
-    for (int k = 0; k < FOURS; ++k)
+  for (int k = 0; k < FOURS; ++k)
 #pragma unroll
-      for (int e = 0; e < 4; ++e) acc[k][e] = 0.f;
-    if (live) {
+    for (int e = 0; e < 4; ++e) acc[k][e] = 0.f;
+  auto power = [&](float x) { return base2 ? exp2f(x) : expf(x); };
+  if (live && four0 < fours) {
 #pragma unroll 2
-      for (int c = c0 + (MANY ? warp : 0); c <= c1; c += MANY ? WARPS : 1) {
-        const size_t s = slot_of(c);
-        const float2 ml = part_ml[s * sh.rows_block + r];
-        float4 o[FOURS];
+    for (int c = c0 + part_group; c <= c1; c += PARTS) {
+      const size_t s = 2 * ((size_t)c * sh.split + row_block % sh.split) + (c == c0 ? 1 : 0);
+      const float2 ml = part_ml[s * sh.rows_block + r];
+      float4 o[FOURS];
 #pragma unroll
-        for (int k = 0; k < FOURS; ++k)
-          if (four0 + k < fours) o[k] = part_o[part_at(sh, s, fours, four0 + k, r)];
-        const float w = base2 ? exp2f(ml.x - ref) : expf(ml.x - ref);
-        l += w * ml.y;
+      for (int k = 0; k < FOURS; ++k) o[k] = four0 + k < fours ? part_o[part_at(sh, s, fours, four0 + k, r)] : make_float4(0.f, 0.f, 0.f, 0.f);
+      const float m_new = fmaxf(m, ml.x), ref = m_new == -INFINITY ? 0.f : m_new;
+      const float was = power(m - ref), is = power(ml.x - ref);
+      m = m_new;
+      l = l * was + ml.y * is;
 #pragma unroll
-        for (int k = 0; k < FOURS; ++k)
-          if (four0 + k < fours && w != 0.f) {
-            acc[k][0] = fmaf(w, o[k].x, acc[k][0]);
-            acc[k][1] = fmaf(w, o[k].y, acc[k][1]);
-            acc[k][2] = fmaf(w, o[k].z, acc[k][2]);
-            acc[k][3] = fmaf(w, o[k].w, acc[k][3]);
-          }
+      for (int k = 0; k < FOURS; ++k) {
+        acc[k][0] = acc[k][0] * was + o[k].x * is;
+        acc[k][1] = acc[k][1] * was + o[k].y * is;
+        acc[k][2] = acc[k][2] * was + o[k].z * is;
+        acc[k][3] = acc[k][3] * was + o[k].w * is;
       }
     }
-    if (MANY) {
-#pragma unroll
-      for (int k = 0; k < FOURS; ++k)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) s_acc[warp][k * 4 + e][lane] = acc[k][e];
-      s_acc[warp][FOURS * 4][lane] = l;
-      __syncthreads();
-      if (warp != 0) return;
-#pragma unroll
-      for (int k = 0; k < FOURS; ++k)
-#pragma unroll
-        for (int e = 0; e < 4; ++e)
-          for (int w = 1; w < WARPS; ++w) acc[k][e] += s_acc[w][k * 4 + e][lane];
-      for (int w = 1; w < WARPS; ++w) l += s_acc[w][FOURS * 4][lane];
-    }
-    const float inv = l == 0.f ? 0.f : 1.0f / l;
-    if (live) {
-#pragma unroll
-      for (int k = 0; k < FOURS; ++k)
-#pragma unroll
-        for (int e = 0; e < 4; ++e)
-          if ((four0 + k) * 4 + e < hd) gi::stf(dst + (four0 + k) * 4 + e, acc[k][e] * inv);
-    }
   }
+#pragma unroll
+  for (int k = 0; k < FOURS; ++k)
+#pragma unroll
+    for (int e = 0; e < 4; ++e) s_acc[warp][k * 4 + e][lane] = acc[k][e];
+  s_acc[warp][FOURS * 4][lane] = m;
+  s_acc[warp][FOURS * 4 + 1][lane] = l;
+  __syncthreads();
+  // a cut's 16 numbers of 32 rows: PARTS warps' results, added up by those warps, 16 / PARTS numbers each
+  const int w0 = warp / PARTS * PARTS;
+  float top = -INFINITY, weight[PARTS];
+#pragma unroll
+  for (int w = 0; w < PARTS; ++w) top = fmaxf(top, s_acc[w0 + w][FOURS * 4][lane]);
+  l = 0.f;
+#pragma unroll
+  for (int w = 0; w < PARTS; ++w) {
+    weight[w] = power(s_acc[w0 + w][FOURS * 4][lane] - (top == -INFINITY ? 0.f : top));
+    l += weight[w] * s_acc[w0 + w][FOURS * 4 + 1][lane];
+  }
+  const float inv = l == 0.f ? 0.f : 1.0f / l;
+  if (!live) return;
+  T* dst = out + (size_t)(tok0 + row / group) * ldo + (size_t)(kvh * group + row % group) * hd;
+  constexpr int EACH = FOURS * 4 / PARTS;
+  float o[EACH];
+#pragma unroll
+  for (int e = 0; e < EACH; ++e) {
+    o[e] = 0.f;
+#pragma unroll
+    for (int w = 0; w < PARTS; ++w) o[e] += weight[w] * s_acc[w0 + w][part_group * EACH + e][lane];
+  }
+  const int d0 = four0 * 4 + part_group * EACH;
+#pragma unroll
+  for (int e = 0; e < EACH; ++e)
+    if (d0 + e < hd) gi::stf(dst + d0 + e, o[e] * inv);
 }
 
 struct Plan {
   int ranges, split, rows_block, tile, least;
-  bool many_parts;      // a unit may lie on more blocks than one warp should join
+  bool many_parts;      // a unit lies on more than a few blocks
 };
 
 // The query rows of a block: 16 or 64 on CUDA cores, the smaller where it takes a tree's rows; on tensor cores as many whole nodes as
@@ -312,7 +314,7 @@ Plan plan_of(int n_seqs, int max_nodes, int max_kv_len, int n_heads, int n_kv, b
   const long cap = (tensor ? 1L : 2L) * gi::sm_count() / p.split;
   p.ranges = (int)(wanted < cap ? wanted : cap);
   if (p.ranges < 1) p.ranges = 1;
-  p.many_parts = p.ranges > 16 * units;
+  p.many_parts = p.ranges > 3 * units;
   return p;
 }
 
@@ -388,8 +390,9 @@ extern "C" int gi_attn_tree(void* out, long ldo, const void* q, long ldq, long q
     GI_DISPATCH_DTYPE(dtype, T, rc = (launch_tree_dims<T, 16>(sh, p, (T*)out, ldo, (const T*)q, ldq, (const T*)kcache, (const T*)vcache, hd, scale, part_o, part_ml, prefix_out, s)));
   if (rc != GI_OK) return rc;
   const int rows = max_nodes * (n_heads / n_kv);
-  const dim3 join((unsigned)((rows + 31) / 32 * (p.many_parts ? (hd + 15) / 16 : 1)), n_kv, n_seqs);
-  GI_DISPATCH_DTYPE(dtype, T, rc = gi::check(gi::launch(p.many_parts ? attn_tree_join_kernel<T, true> : attn_tree_join_kernel<T, false>, join, dim3(THREADS), 0, s, sh,
-                                                        (T*)out, ldo, hd, p.ranges, tensor ? 1 : 0, part_o, part_ml, prefix_out), "tree attention (join)"));
+  const int numbers = p.many_parts ? 16 : 64;               // of a head, in a block of the join
+  const dim3 join((unsigned)((rows + 31) / 32 * ((hd + numbers - 1) / numbers)), n_kv, n_seqs);
+  GI_DISPATCH_DTYPE(dtype, T, rc = gi::check(gi::launch(p.many_parts ? attn_tree_join_kernel<T, 8> : attn_tree_join_kernel<T, 2>, join, dim3(THREADS), 0, s, sh, (T*)out,
+                                                        ldo, hd, p.ranges, tensor ? 1 : 0, part_o, part_ml, prefix_out), "tree attention (join)"));
   return rc;
 }
