@@ -206,13 +206,47 @@ attn_tree_kernel(const Shape sh, T* __restrict__ out, long ldo, const T* q, long
   }
 }
 
+// N neighbouring numbers, in as few stores as their type allows where the rows are aligned to them.
+template <int N>
+__device__ __forceinline__ void store_row(float* dst, const float (&o)[N], int count, bool vec) {
+  if (vec && count >= N) {
+    if constexpr (N >= 4) {
+#pragma unroll
+      for (int e = 0; e < N; e += 4) gi::st4(dst + e, make_float4(o[e], o[e + 1], o[e + 2], o[e + 3]));
+    } else {
+      *reinterpret_cast<float2*>(dst) = make_float2(o[0], o[1]);
+    }
+    return;
+  }
+#pragma unroll
+  for (int e = 0; e < N; ++e)
+    if (e < count) dst[e] = o[e];
+}
+template <int N>
+__device__ __forceinline__ void store_row(__nv_bfloat16* dst, const float (&o)[N], int count, bool vec) {
+  if (vec && count >= N) {
+    uint32_t w[N / 2];
+#pragma unroll
+    for (int e = 0; e < N; e += 2) {
+      const __nv_bfloat162 v = __floats2bfloat162_rn(o[e], o[e + 1]);
+      w[e / 2] = *reinterpret_cast<const uint32_t*>(&v);
+    }
+    if constexpr (N == 8) *reinterpret_cast<uint4*>(dst) = make_uint4(w[0], w[1], w[2], w[3]);
+    else *reinterpret_cast<uint32_t*>(dst) = w[0];
+    return;
+  }
+#pragma unroll
+  for (int e = 0; e < N; ++e)
+    if (e < count) gi::stf(dst + e, o[e]);
+}
+
 // Joins the parts of the units that several blocks hold; maxima are in units of ln, or of powers of two (base2).  A block takes 32
 // query rows of a kv head, one to a lane, and 16 of the head's numbers for each of WARPS / PARTS warps; PARTS warps share out a
 // row's parts.  A part's maximum, sum and values are asked for together and joined as they come (one trip to memory, not one
 // for the maxima and then one for the values); the warps meet in shared memory.
 template <typename T, int PARTS>
 __global__ void __launch_bounds__(THREADS)
-attn_tree_join_kernel(const Shape sh, T* __restrict__ out, long ldo, int hd, int ranges, int base2, const float4* part_o, const float2* part_ml,
+attn_tree_join_kernel(const Shape sh, T* __restrict__ out, long ldo, int hd, int ranges, int base2, int vec, const float4* part_o, const float2* part_ml,
                       const int* part_prefix) {
   constexpr int WARPS = THREADS / 32, CUTS = WARPS / PARTS, FOURS = 4;      // pieces of four numbers that a thread holds
   __shared__ float s_acc[WARPS][FOURS * 4 + 2][33];
@@ -286,10 +320,10 @@ attn_tree_join_kernel(const Shape sh, T* __restrict__ out, long ldo, int hd, int
 #pragma unroll
     for (int w = 0; w < PARTS; ++w) o[e] += weight[w] * s_acc[w0 + w][part_group * EACH + e][lane];
   }
-  const int d0 = four0 * 4 + part_group * EACH;
 #pragma unroll
-  for (int e = 0; e < EACH; ++e)
-    if (d0 + e < hd) gi::stf(dst + d0 + e, o[e] * inv);
+  for (int e = 0; e < EACH; ++e) o[e] *= inv;
+  const int d0 = four0 * 4 + part_group * EACH;
+  store_row<EACH>(dst + d0, o, hd - d0, vec != 0);
 }
 
 struct Plan {
@@ -390,9 +424,10 @@ extern "C" int gi_attn_tree(void* out, long ldo, const void* q, long ldq, long q
     GI_DISPATCH_DTYPE(dtype, T, rc = (launch_tree_dims<T, 16>(sh, p, (T*)out, ldo, (const T*)q, ldq, (const T*)kcache, (const T*)vcache, hd, scale, part_o, part_ml, prefix_out, s)));
   if (rc != GI_OK) return rc;
   const int rows = max_nodes * (n_heads / n_kv);
+  const int vec = hd % 8 == 0 && ldo % 8 == 0 && ((uintptr_t)out & 15) == 0;
   const int numbers = p.many_parts ? 16 : 64;               // of a head, in a block of the join
   const dim3 join((unsigned)((rows + 31) / 32 * ((hd + numbers - 1) / numbers)), n_kv, n_seqs);
   GI_DISPATCH_DTYPE(dtype, T, rc = gi::check(gi::launch(p.many_parts ? attn_tree_join_kernel<T, 8> : attn_tree_join_kernel<T, 2>, join, dim3(THREADS), 0, s, sh, (T*)out,
-                                                        ldo, hd, p.ranges, tensor ? 1 : 0, part_o, part_ml, prefix_out), "tree attention (join)"));
+                                                        ldo, hd, p.ranges, tensor ? 1 : 0, vec, part_o, part_ml, prefix_out), "tree attention (join)"));
   return rc;
 }
