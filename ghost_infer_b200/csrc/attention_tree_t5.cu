@@ -2,8 +2,8 @@
 //
 // The query rows of a kv head (its group's heads x a tree's nodes) share every key and value: a block takes up to 128 of them (whole
 // nodes, one query row to a lane of tensor memory) and walks its range of 128-key tiles (attention_tree.cuh).  One warp fetches
-// queries, and keys and values page by page, with TMA; one thread issues the score products S = Q K^T into one of two score
-// buffers, another one the output products O += P V with P read from tensor memory.  Eight warps make the probabilities: a row
+// queries and, page by page, keys with TMA, another one values; one thread issues the score products S = Q K^T into one of two score
+// buffers, a second one the output products O += P V with P read from tensor memory.  Eight warps make the probabilities: a row
 // is two threads' work, one for the first 64 keys of every tile and one for the second.  The two know nothing of each other
 // until the end: each has a running maximum and sum (32 bits, base-2 exponentials) and an accumulator of its own in tensor
 // memory, rescaled when its reference point moves by more than 2^8, and writes its probabilities as bfloat16 over the scores
@@ -101,11 +101,11 @@ struct Layout {
   static constexpr uint32_t STATS_AT = FLAGS_AT + 4 * 8 + 16;                          // [this unit's, the last one's][2][128] maximum and sum
   static constexpr uint32_t PREFIX_AT = STATS_AT + 4 * BQ * 8;
   static constexpr uint32_t BYTES = PREFIX_AT + 4 * (MAX_SEQS + 1);
-  static constexpr int ROW_THREADS = 256, THREADS = ROW_THREADS + 96, COLS = 512;
+  static constexpr int ROW_THREADS = 256, THREADS = ROW_THREADS + 128, COLS = 512;
 };
 
 template <int HALVES, int STAGES>
-__global__ void __launch_bounds__(352, 1)
+__global__ void __launch_bounds__(384, 1)
 attn_tree_t5_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v,
                     const __grid_constant__ Shape sh, __nv_bfloat16* __restrict__ out, long ldo, float scale, int q_box, float4* __restrict__ part_o,
                     float2* __restrict__ part_ml, int* __restrict__ part_prefix) {
@@ -179,11 +179,15 @@ attn_tree_t5_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
   int at = lo, t_begin, t_end;
   Unit u;
 
-  if (warp == 8) {
-    // ---- queries; keys and values: the pages of 16 tiles are looked up side by side
+  if (warp == 8 || warp == 11) {
+    // ---- warp 8: queries and keys, warp 11: values (one warp for both would ask for keys only when the values' stage before them is
+    // free, a whole tile late).  The pages of 16 tiles are looked up side by side.
+    const bool keys = warp == 8;
+    const CUtensorMap* map = keys ? &map_k : &map_v;
+    const uint32_t full = keys ? k_full : v_full, empty = keys ? k_empty : v_empty, stages = smem_u32(smem + (keys ? L::K_AT : L::V_AT));
     for (; ok && next_unit(at, u, t_begin, t_end); ++f) {
       const int pages = (u.pos0 + u.n + PAGE_TOKENS - 1) / PAGE_TOKENS;
-      if (lane == 0) {
+      if (keys && lane == 0) {
         if (f > 0) ok = mbar_wait(q_empty, (uint32_t)((f - 1) & 1), 1, &g_tree_status);
         if (ok) {
           // rows of a box: a node's heads one below the other (a row past the sequence's nodes belongs to nobody and is not looked at)
@@ -203,27 +207,15 @@ attn_tree_t5_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
           const int row[2] = {__shfl_sync(0xffffffffu, mine, 2 * i), __shfl_sync(0xffffffffu, mine, 2 * i + 1)};
           const int s = j % STAGES;
           if (lane == 0) {
-            const uint32_t parity = (uint32_t)((j / STAGES - 1) & 1);
-            if (j >= STAGES) ok = mbar_wait(k_empty + 8 * s, parity, 1, &g_tree_status);
+            if (j >= STAGES) ok = mbar_wait(empty + 8 * s, (uint32_t)((j / STAGES - 1) & 1), 1, &g_tree_status);
             if (ok) {
-              mbar_expect_tx(k_full + 8 * s, L::BYTES_TILE);
+              mbar_expect_tx(full + 8 * s, L::BYTES_TILE);
 #pragma unroll
               for (int x = 0; x < 2 * HALVES; ++x)
-                tma_load_2d(smem_u32(smem + L::K_AT + s * L::BYTES_TILE + (x >> 1) * HALF + (x & 1) * (HALF / 2)), &map_k, (x >> 1) * 64, row[x & 1], k_full + 8 * s);
-              if (j >= STAGES) ok = mbar_wait(v_empty + 8 * s, parity, 1, &g_tree_status);
-            }
-            if (ok) {
-              mbar_expect_tx(v_full + 8 * s, L::BYTES_TILE);
-#pragma unroll
-              for (int x = 0; x < 2 * HALVES; ++x)
-                tma_load_2d(smem_u32(smem + L::V_AT + s * L::BYTES_TILE + (x >> 1) * HALF + (x & 1) * (HALF / 2)), &map_v, (x >> 1) * 64, row[x & 1], v_full + 8 * s);
+                tma_load_2d(stages + s * L::BYTES_TILE + (x >> 1) * HALF + (x & 1) * (HALF / 2), map, (x >> 1) * 64, row[x & 1], full + 8 * s);
             } else {
-              // giving up: the copies under way must have landed before the block's shared memory goes to another one.  The last
-              // copy of keys may be tile j's, that of values tile j - 1's
-              for (int t = max(0, j - STAGES); t <= j; ++t) {
-                if (t > j - STAGES) mbar_wait(k_full + 8 * (t % STAGES), (uint32_t)((t / STAGES) & 1), 1, &g_tree_status);
-                if (t < j) mbar_wait(v_full + 8 * (t % STAGES), (uint32_t)((t / STAGES) & 1), 1, &g_tree_status);
-              }
+              // giving up: the copies under way must have landed before the block's shared memory goes to another one
+              for (int t = max(0, j - STAGES); t < j; ++t) mbar_wait(full + 8 * (t % STAGES), (uint32_t)((t / STAGES) & 1), 1, &g_tree_status);
             }
           }
           ok = __shfl_sync(0xffffffffu, ok ? 1 : 0, 0) != 0;
