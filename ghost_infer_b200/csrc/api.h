@@ -679,18 +679,16 @@ long gi_beam_select_scratch(int rows, int vocab, int width);
 int gi_beam_select(float* out_scores, int* out_parents, int* out_tokens, const void* logits, int dtype, long ld, const float* scores,
                    int seqs, int beams, int vocab, int width, void* scratch, long scratch_bytes, void* stream);
 
-// Fixed-size states take their beams' parents' place, in place: in each of `n` tensors (host arrays of addresses and row sizes; a
-// tensor has `rows` rows one after the other) row slots[s][j] becomes what row slots[s][parents[s][j]] held before the call.  The
+// Fixed-size states take their beams' parents' place, in place: in each of `n` tensors (host array of two words each, address and bytes of a
+// row; a tensor has `rows` rows one after the other) row slots[s][j] becomes what row slots[s][parents[s][j]] held before the call.  The
 // slots of a call are distinct.  A slot outside [0, rows) or a parent outside [0, beams) leaves its row as it is.  beams 1 to
 // 64; unit 16, 4 or 1: bytes that every address and row size is a multiple of.
-int gi_reorder_states(void* const* states, const long* row_bytes, int n, int unit, const int* slots, const int* parents, int seqs,
-                      int beams, int rows, void* stream);
+int gi_reorder_states(const long* states, int n, int unit, const int* slots, const int* parents, int seqs, int beams, int rows, void* stream);
 
 // The first rows[i] (null: all 64) positions of page src[i] are copied to page dst[i] for every layer and head of `n` (at most 8)
-// tensors [layers][pages][heads][64][row bytes] (host arrays).  No page that is written is read or written twice in one call.
+// tensors [layers][pages][heads][64][row bytes] (host array of five words each: address, layers, pages, heads, row bytes).  No page that is written is read or written twice in one call.
 // Pages outside a tensor are passed over.
-int gi_copy_pages(void* const* tensors, const int* layers, const int* pages, const int* heads, const int* row_bytes, int n,
-                  const int* src, const int* dst, const int* rows, int copies, void* stream);
+int gi_copy_pages(const long* tensors, int n, const int* src, const int* dst, const int* rows, int copies, void* stream);
 
 // Attention of drafted tokens: the tokens of sequence b (cu_seqlens, at most max_nodes <= 256 of them, the rest is left out) are the
 // nodes of a tree whose keys and values lie at the positions seq_pos0[b] + node of the cache already; a node sees every position
@@ -712,9 +710,8 @@ int gi_attn_tree_status(int* status);
 // seq_pos0 + node to seq_pos0 + place in the path, in every layer and head of `n` (0 to 8) tensors of pages (as gi_copy_pages).
 // A slot of -1 moves nothing; positions outside the table or pages outside a tensor are passed over.  max_nodes 1 to 256.
 int gi_tree_commit(int* out_path, int* out_counts, int* out_next, const int* picks, const int* tokens, const int* parents,
-                   const int* cu_seqlens, const int* seq_slots, const int* seq_pos0, int n_seqs, int max_nodes, void* const* tensors,
-                   const int* layers, const int* pages, const int* heads, const int* row_bytes, int n, const int* block_table,
-                   int max_pages, void* stream);
+                   const int* cu_seqlens, const int* seq_slots, const int* seq_pos0, int n_seqs, int max_nodes, const long* tensors,
+                   int n, const int* block_table, int max_pages, void* stream);
 
 #ifdef __cplusplus
 }

@@ -12,6 +12,7 @@
 // Both are bound by the bytes they move.
 #include "api.h"
 #include "common.cuh"
+#include "page_tensors.cuh"
 
 namespace {
 
@@ -125,16 +126,9 @@ int launch_states(const StateTensors& t, int n, const int* slots, const int* par
   return gi::check(gi::launch(kern, grid(1), dim3(THREADS), smem, s, t, slots, parents, beams, rows), "state reordering");
 }
 
-constexpr int MAX_PAGE_TENSORS = 8;
-struct PageTensors {
-  void* base[MAX_PAGE_TENSORS];
-  int layers[MAX_PAGE_TENSORS], heads[MAX_PAGE_TENSORS], row_units[MAX_PAGE_TENSORS];    // [layers][pages][heads][64][row units]
-  int pages[MAX_PAGE_TENSORS];
-};
-
 template <typename V>
 __global__ void __launch_bounds__(THREADS)
-copy_pages_kernel(const __grid_constant__ PageTensors t, const int* src, const int* dst, const int* rows, int copies) {
+copy_pages_kernel(const __grid_constant__ gi::PageTensors t, const int* src, const int* dst, const int* rows, int copies) {
   constexpr int AHEAD = 4;
   const int z = blockIdx.z, layer = blockIdx.x / t.heads[z], head = blockIdx.x % t.heads[z];
   gi::pdl_prologue();
@@ -160,8 +154,7 @@ copy_pages_kernel(const __grid_constant__ PageTensors t, const int* src, const i
 
 }  // namespace
 
-extern "C" int gi_reorder_states(void* const* states, const long* row_bytes, int n, int unit, const int* slots, const int* parents, int seqs,
-                                 int beams, int rows, void* stream) {
+extern "C" int gi_reorder_states(const long* states, int n, int unit, const int* slots, const int* parents, int seqs, int beams, int rows, void* stream) {
   if (seqs <= 0 || n <= 0) return GI_OK;
   if (beams < 1 || beams > MAX_BEAMS) return gi::fail(GI_ERR_ARG, "state reordering: %d beams, 1 to %d are supported", beams, MAX_BEAMS);
   if (seqs > 65535) return gi::fail(GI_ERR_UNSUPPORTED, "state reordering: more than 65535 sequences in one launch");
@@ -171,10 +164,11 @@ extern "C" int gi_reorder_states(void* const* states, const long* row_bytes, int
     StateTensors t = {};
     const int here = n - first < MAX_TENSORS ? n - first : MAX_TENSORS;
     for (int i = 0; i < here; ++i) {
-      if (row_bytes[first + i] < 1 || row_bytes[first + i] % unit != 0 || ((uintptr_t)states[first + i] % unit) != 0)
-        return gi::fail(GI_ERR_ARG, "state reordering: rows of %ld bytes do not come in units of %d", row_bytes[first + i], unit);
-      t.base[i] = states[first + i];
-      t.units[i] = row_bytes[first + i] / unit;
+      const long address = states[2 * (first + i)], row_bytes = states[2 * (first + i) + 1];
+      if (row_bytes < 1 || row_bytes % unit != 0 || address % unit != 0)
+        return gi::fail(GI_ERR_ARG, "state reordering: rows of %ld bytes do not come in units of %d", row_bytes, unit);
+      t.base[i] = (void*)address;
+      t.units[i] = row_bytes / unit;
     }
     cudaStream_t s = (cudaStream_t)stream;
     const int rc = unit == 16 ? launch_states<uint4>(t, here, slots, parents, seqs, beams, rows, s)
@@ -185,22 +179,15 @@ extern "C" int gi_reorder_states(void* const* states, const long* row_bytes, int
   return GI_OK;
 }
 
-extern "C" int gi_copy_pages(void* const* tensors, const int* layers, const int* pages, const int* heads, const int* row_bytes, int n,
-                             const int* src, const int* dst, const int* rows, int copies, void* stream) {
+extern "C" int gi_copy_pages(const long* tensors, int n, const int* src, const int* dst, const int* rows, int copies, void* stream) {
   if (copies <= 0 || n <= 0) return GI_OK;
-  if (n > MAX_PAGE_TENSORS) return gi::fail(GI_ERR_UNSUPPORTED, "page copies: more than %d tensors in one launch", MAX_PAGE_TENSORS);
-  int unit = 16;
+  gi::PageTensors t;
+  int unit;
+  const int rc = t.read(tensors, n, &unit, "page copies");
+  if (rc != GI_OK) return rc;
   long most = 0;
-  for (int i = 0; i < n; ++i) {
-    if (layers[i] < 1 || pages[i] < 1 || heads[i] < 1 || row_bytes[i] < 2 || row_bytes[i] % 2 != 0 || ((uintptr_t)tensors[i] & 1))
-      return gi::fail(GI_ERR_ARG, "page copies: tensor %d has %d layers, %d pages, %d heads, rows of %d bytes", i, layers[i], pages[i], heads[i], row_bytes[i]);
-    // 64 rows of any even number of bytes are a multiple of 16; a copy's end need not be
-    while (unit > 2 && (row_bytes[i] % unit != 0 || ((uintptr_t)tensors[i] % unit) != 0)) unit = unit == 16 ? 4 : 2;
-    most = (long)layers[i] * heads[i] > most ? (long)layers[i] * heads[i] : most;
-  }
+  for (int i = 0; i < n; ++i) most = (long)t.layers[i] * t.heads[i] > most ? (long)t.layers[i] * t.heads[i] : most;
   if (most > 0x7fffffffL) return gi::fail(GI_ERR_UNSUPPORTED, "page copies: more than 2^31 - 1 heads of all layers");
-  PageTensors t = {};
-  for (int i = 0; i < n; ++i) t.base[i] = tensors[i], t.layers[i] = layers[i], t.pages[i] = pages[i], t.heads[i] = heads[i], t.row_units[i] = row_bytes[i] / unit;
   const dim3 grid((unsigned)most, copies < 65535 ? copies : 65535, n);
   cudaStream_t s = (cudaStream_t)stream;
   if (unit == 16) return gi::check(gi::launch(copy_pages_kernel<uint4>, grid, dim3(THREADS), 0, s, t, src, dst, rows, copies), "page copies");

@@ -423,6 +423,16 @@ int gi::tensor_map_2d_ex(CUtensorMap* out, const void* base, long rows, long col
 }
 
 int gi::tensor_map_3d(CUtensorMap* out, const void* base, long rows, long heads, long cols, long row_ld, long head_ld, int box_cols, int box_heads, int box_rows) {
+  typedef std::tuple<const void*, long, long, long, long, long, int, int, int> Key;
+  static std::map<Key, CUtensorMap> cache;
+  static std::mutex lock;
+  const Key key(base, rows, heads, cols, row_ld, head_ld, box_cols, box_heads, box_rows);
+  std::lock_guard<std::mutex> guard(lock);
+  auto it = cache.find(key);
+  if (it != cache.end()) {
+    *out = it->second;
+    return GI_OK;
+  }
   EncodeTiled enc = encoder();
   if (!enc) return gi::fail(GI_ERR_CUDA, "tensor map: the driver does not export cuTensorMapEncodeTiled");
   const cuuint64_t dims[3] = {(cuuint64_t)cols, (cuuint64_t)heads, (cuuint64_t)rows};
@@ -432,6 +442,8 @@ int gi::tensor_map_3d(CUtensorMap* out, const void* base, long rows, long heads,
   CUresult r = enc(out, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, const_cast<void*>(base), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
                    CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   if (r != CUDA_SUCCESS) return gi::fail(GI_ERR_CUDA, "tensor map of three dimensions: cuTensorMapEncodeTiled failed with %d", (int)r);
+  if (cache.size() > 4096) cache.clear();
+  cache[key] = *out;
   return GI_OK;
 }
 

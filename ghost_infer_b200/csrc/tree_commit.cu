@@ -11,22 +11,15 @@
 // costs less than a launch of its own that the moves would wait for.  Bound: latency; the moved rows' bytes for many sequences.
 #include "api.h"
 #include "common.cuh"
+#include "page_tensors.cuh"
 
 namespace {
 
 constexpr int THREADS = 256;
 constexpr int MAX_NODES = 256;
-constexpr int MAX_PAGE_TENSORS = 8;
-
-struct TreeTensors {
-  void* base[MAX_PAGE_TENSORS];
-  int layers[MAX_PAGE_TENSORS], pages[MAX_PAGE_TENSORS], heads[MAX_PAGE_TENSORS], row_units[MAX_PAGE_TENSORS];
-  long columns[MAX_PAGE_TENSORS];    // layers * heads * row units
-};
-
 template <typename V>
 __global__ void __launch_bounds__(THREADS)
-tree_commit_kernel(const __grid_constant__ TreeTensors t, int n_tensors, const int* picks, const int* tokens, const int* parents,
+tree_commit_kernel(const __grid_constant__ gi::PageTensors t, int n_tensors, const int* picks, const int* tokens, const int* parents,
                    const int* cu_seqlens, const int* seq_slots, const int* seq_pos0, const int* block_table, int max_pages, int max_nodes,
                    int* __restrict__ out_path, int* __restrict__ out_counts, int* __restrict__ out_next) {
   __shared__ int s_token[MAX_NODES], s_parent[MAX_NODES], s_pick[MAX_NODES], s_path[MAX_NODES], s_page[MAX_NODES / PAGE_TOKENS + 2];
@@ -78,7 +71,8 @@ tree_commit_kernel(const __grid_constant__ TreeTensors t, int n_tensors, const i
 
   long col = (long)blockIdx.x * THREADS + tid;
   int z = 0;
-  while (z < n_tensors && col >= t.columns[z]) col -= t.columns[z++];
+  auto columns = [&](int i) { return (long)t.layers[i] * t.heads[i] * t.row_units[i]; };
+  while (z < n_tensors && col >= columns(z)) col -= columns(z++);
   if (z >= n_tensors) return;
   const int ru = t.row_units[z], c = (int)(col % ru), head = (int)(col / ru % t.heads[z]), layer = (int)(col / ru / t.heads[z]);
   V* base = (V*)t.base[z];
@@ -113,25 +107,17 @@ tree_commit_kernel(const __grid_constant__ TreeTensors t, int n_tensors, const i
 }  // namespace
 
 extern "C" int gi_tree_commit(int* out_path, int* out_counts, int* out_next, const int* picks, const int* tokens, const int* parents,
-                              const int* cu_seqlens, const int* seq_slots, const int* seq_pos0, int n_seqs, int max_nodes, void* const* tensors,
-                              const int* layers, const int* pages, const int* heads, const int* row_bytes, int n, const int* block_table,
-                              int max_pages, void* stream) {
+                              const int* cu_seqlens, const int* seq_slots, const int* seq_pos0, int n_seqs, int max_nodes, const long* tensors,
+                              int n, const int* block_table, int max_pages, void* stream) {
   if (n_seqs <= 0) return GI_OK;
   if (max_nodes < 1 || max_nodes > MAX_NODES) return gi::fail(GI_ERR_ARG, "tree commit: trees of up to %d nodes, 1 to %d are supported", max_nodes, MAX_NODES);
   if (n_seqs > 65535) return gi::fail(GI_ERR_UNSUPPORTED, "tree commit: more than 65535 sequences in one launch");
-  if (n < 0 || n > MAX_PAGE_TENSORS) return gi::fail(GI_ERR_UNSUPPORTED, "tree commit: %d tensors of pages, at most %d in one launch", n, MAX_PAGE_TENSORS);
-  int unit = 16;
-  for (int i = 0; i < n; ++i) {
-    if (layers[i] < 1 || pages[i] < 1 || heads[i] < 1 || row_bytes[i] < 2 || row_bytes[i] % 2 != 0 || ((uintptr_t)tensors[i] & 1))
-      return gi::fail(GI_ERR_ARG, "tree commit: tensor %d has %d layers, %d pages, %d heads, rows of %d bytes", i, layers[i], pages[i], heads[i], row_bytes[i]);
-    while (unit > 2 && (row_bytes[i] % unit != 0 || ((uintptr_t)tensors[i] % unit) != 0)) unit = unit == 16 ? 4 : 2;
-  }
-  TreeTensors t = {};
+  gi::PageTensors t;
+  int unit;
+  const int rc = t.read(tensors, n, &unit, "tree commit");
+  if (rc != GI_OK) return rc;
   long columns = 0;
-  for (int i = 0; i < n; ++i) {
-    t.base[i] = tensors[i], t.layers[i] = layers[i], t.pages[i] = pages[i], t.heads[i] = heads[i], t.row_units[i] = row_bytes[i] / unit;
-    columns += t.columns[i] = (long)layers[i] * heads[i] * (row_bytes[i] / unit);
-  }
+  for (int i = 0; i < n; ++i) columns += (long)t.layers[i] * t.heads[i] * t.row_units[i];
   const long blocks = columns > 0 ? (columns + THREADS - 1) / THREADS : 1;
   if (blocks > 0x7fffffffL) return gi::fail(GI_ERR_UNSUPPORTED, "tree commit: more rows' columns than one launch holds");
   const dim3 grid((unsigned)blocks, n_seqs);

@@ -11,6 +11,7 @@ import contextlib
 import contextvars
 import ctypes
 import os
+import struct
 import weakref
 from ctypes import c_float, c_int, c_long, c_void_p
 from typing import Dict, Optional, Tuple
@@ -156,12 +157,12 @@ def _bind():
         "gi_linear_state_keyed": [P, P, L, P, L, P, L, I, P, F, P, L, I, P, P, I, I, I, I, I, P],
         "gi_beam_select": [P, P, P, P, I, L, P, I, I, I, I, P, L, P],
         "gi_beam_select_scratch": [I, I, I],
-        "gi_reorder_states": [P, P, I, I, P, P, I, I, I, P],
-        "gi_copy_pages": [P, P, P, P, P, I, P, P, P, I, P],
+        "gi_reorder_states": [P, I, I, P, P, I, I, I, P],
+        "gi_copy_pages": [P, I, P, P, P, I, P],
         "gi_attn_tree": [P, L, P, L, L, I, P, P, I, P, I, P, P, P, P, I, I, I, I, I, I, I, F, P, L, P],
         "gi_attn_tree_scratch": [I, I, I, I, I, I, I],
         "gi_attn_tree_status": [P],
-        "gi_tree_commit": [P, P, P, P, P, P, P, P, P, I, I, P, P, P, P, P, I, P, I, P],
+        "gi_tree_commit": [P, P, P, P, P, P, P, P, P, I, I, P, I, P, I, P],
         "gi_attn_decode_generic_ex3": [P, L, P, P, P, L, I, P, P, P, I, P, P, I, I, I, I, F, I, I, I, I, F, P, I, L, I, P],
     }
     for name, argtypes in sigs.items():
@@ -2896,19 +2897,28 @@ def linear_state_keyed(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, decay:
 MAX_BEAMS, MAX_BEAM_WIDTH, MAX_TREE_NODES = 64, 64, 256
 
 
-def _on_here(what: str, *tensors: torch.Tensor) -> None:
-    """Refuses tensors that do not live on the current device: the launch goes to that device's current stream."""
-    here = torch.cuda.current_device() if torch.cuda.is_available() else -1
-    for t in tensors:
-        if not t.is_cuda:
-            raise KernelError(f"{what} must live on a CUDA device; there is no CPU path")
-        if t.device.index != here:
-            raise KernelError(f"{what}: a tensor lives on {t.device}, the current device is cuda:{here}")
+def _on_here(what: str, first: torch.Tensor, *others: torch.Tensor) -> int:
+    """The current stream, after a look at the tensors: all live on the current device, whose stream the launch goes to."""
+    device = first.get_device()
+    for t in others:
+        if t.get_device() != device:
+            raise KernelError(f"{what}: tensors on {first.device} and on {t.device}")
+    if device < 0:
+        raise KernelError(f"{what} must live on a CUDA device; there is no CPU path")
+    if device != torch.cuda.current_device():
+        raise KernelError(f"{what}: the tensors live on {first.device}, the current device is cuda:{torch.cuda.current_device()}")
+    return torch._C._cuda_getCurrentRawStream(device)
 
 
 def _i32_of(t: torch.Tensor, n: int, what: str) -> int:
-    if t.dtype != torch.int32 or not t.is_contiguous() or t.numel() != n:
+    if t.dtype is not torch.int32 or t.numel() != n or not t.is_contiguous():
         raise KernelError(f"{what} must be {n} contiguous int32 values, got {t.dtype} {tuple(t.shape)}")
+    return t.data_ptr()
+
+
+def _i32_rows(t: torch.Tensor, what: str) -> int:
+    if t.dtype is not torch.int32 or t.dim() != 2 or not t.is_contiguous():
+        raise KernelError(f"{what} must be a contiguous int32 table, got {t.dtype} {tuple(t.shape)}")
     return t.data_ptr()
 
 
@@ -2919,24 +2929,26 @@ def beam_select(logits: torch.Tensor, scores: torch.Tensor, width: int):
     beam that goes on) and tokens int32, each [sequences, width]; where no candidate is left: -inf, -1, -1.  A logit that is
     no number counts as -inf; a beam whose logits are all -inf or hold a +inf, or whose score is not finite, offers nothing."""
     lib = _bind()
-    _on_here("beam selection", logits, scores)
+    stream = _on_here("beam selection", logits, scores)
     _cuda(logits, "logits")
     ld, dt = _rows(logits, "logits"), _dt(logits, "logits")
-    if scores.dim() != 2 or scores.dtype != torch.float32 or not scores.is_contiguous():
+    if scores.dim() != 2 or scores.dtype is not torch.float32 or not scores.is_contiguous():
         raise KernelError("the beams' scores must be contiguous float32 [sequences, beams]")
     seqs, beams = scores.shape
-    if logits.shape[0] != seqs * beams:
-        raise KernelError(f"{seqs} sequences of {beams} beams want {seqs * beams} rows of logits, got {logits.shape[0]}")
-    vocab, width = logits.shape[1], int(width)
-    out = torch.empty((seqs, width), dtype=torch.float32, device=logits.device) if width > 0 else None
-    if out is None or width > MAX_BEAM_WIDTH or width > beams * vocab:
+    rows, vocab = logits.shape
+    if rows != seqs * beams:
+        raise KernelError(f"{seqs} sequences of {beams} beams want {seqs * beams} rows of logits, got {rows}")
+    if not 1 <= width <= MAX_BEAM_WIDTH or width > beams * vocab:
         raise KernelError(f"a width of {width}: 1 to {MAX_BEAM_WIDTH} and at most beams x vocabulary are supported")
-    picks = torch.empty((2, seqs, width), dtype=torch.int32, device=logits.device)
-    nbytes = lib.gi_beam_select_scratch(seqs * beams, vocab, width)
-    scratch = torch.empty((max(nbytes, 16),), dtype=torch.uint8, device=logits.device)
-    _check(lib, lib.gi_beam_select(out.data_ptr(), picks[0].data_ptr(), picks[1].data_ptr(), logits.data_ptr(), dt, ld, scores.data_ptr(), seqs, beams, vocab,
-                                   width, scratch.data_ptr(), nbytes, _stream()), 2 if seqs else 0)
-    return out, picks[0], picks[1]
+    device = logits.device
+    out = torch.empty((seqs, width), dtype=torch.float32, device=device)
+    parents = torch.empty((seqs, width), dtype=torch.int32, device=device)
+    tokens = torch.empty_like(parents)
+    nbytes = lib.gi_beam_select_scratch(rows, vocab, width)
+    scratch = torch.empty((nbytes,), dtype=torch.uint8, device=device)
+    _check(lib, lib.gi_beam_select(out.data_ptr(), parents.data_ptr(), tokens.data_ptr(), logits.data_ptr(), dt, ld, scores.data_ptr(), seqs, beams, vocab,
+                                   width, scratch.data_ptr(), nbytes, stream), 2 if seqs else 0)
+    return out, parents, tokens
 
 
 def reorder_states(states, slots: torch.Tensor, parents: torch.Tensor) -> None:
@@ -2946,7 +2958,7 @@ def reorder_states(states, slots: torch.Tensor, parents: torch.Tensor) -> None:
     as it is."""
     lib = _bind()
     states = list(states)
-    _on_here("state reordering", slots, parents, *states)
+    stream = _on_here("state reordering", slots, parents, *states)
     if slots.dim() != 2 or slots.shape != parents.shape:
         raise KernelError(f"slots and parents must both be [sequences, beams], got {tuple(slots.shape)} and {tuple(parents.shape)}")
     seqs, beams = slots.shape
@@ -2954,31 +2966,34 @@ def reorder_states(states, slots: torch.Tensor, parents: torch.Tensor) -> None:
         raise KernelError(f"{beams} beams: 1 to {MAX_BEAMS} are supported")
     sp, pp = _i32_of(slots, seqs * beams, "slots"), _i32_of(parents, seqs * beams, "parents")
     by_unit: Dict[int, list] = {}
+    named = set()
     for t in states:
         if t.dim() < 1 or not t.is_contiguous() or t.shape[0] != states[0].shape[0]:
             raise KernelError("states must be contiguous tensors with equally many rows")
-        if t.numel() == 0:
+        size = t.numel()
+        if size == 0:
             continue
-        ptr, row = t.data_ptr(), t.numel() // t.shape[0] * t.element_size()
+        ptr, row = t.data_ptr(), size // t.shape[0] * t.element_size()
+        if ptr in named:
+            raise KernelError("a state is named twice")
+        named.add(ptr)
         both = ptr | row
-        by_unit.setdefault(16 if both % 16 == 0 else (4 if both % 4 == 0 else 1), []).append((ptr, row))
-    if len({p for group in by_unit.values() for p, _ in group}) != sum(len(group) for group in by_unit.values()):
-        raise KernelError("a state is named twice")
-    for unit, group in by_unit.items():
-        n = len(group)
-        ptrs, rows = (c_void_p * n)(*(p for p, _ in group)), (c_long * n)(*(r for _, r in group))
-        _check(lib, lib.gi_reorder_states(ptrs, rows, n, unit, sp, pp, seqs, beams, states[0].shape[0], _stream()), (n + 63) // 64 if seqs else 0)
+        by_unit.setdefault(16 if both % 16 == 0 else (4 if both % 4 == 0 else 1), []).extend((ptr, row))
+    for unit, words in by_unit.items():
+        n = len(words) // 2
+        _check(lib, lib.gi_reorder_states(struct.pack(f"{2 * n}q", *words), n, unit, sp, pp, seqs, beams, states[0].shape[0], stream), (n + 63) // 64 if seqs else 0)
 
 
-def _page_tensors(pages, what: str):
-    """(addresses, layers, pages, heads, row bytes) as C arrays of storage tensors [layers, pages, heads, 64, numbers]."""
+def _page_tensors(pages, what: str) -> bytes:
+    """(address, layers, pages, heads, bytes of a row) of every storage tensor [layers, pages, heads, 64, numbers], as 64-bit words."""
+    words = []
     for t in pages:
-        if t.dim() != 5 or t.shape[3] != 64 or not t.is_contiguous() or t.element_size() not in (2, 4):
+        size = t.element_size()
+        if t.dim() != 5 or t.shape[3] != 64 or size not in (2, 4) or not t.is_contiguous():
             raise KernelError(f"{what}: page storage must be contiguous [layers, pages, heads, 64, numbers] of 2 or 4 bytes a number, got {tuple(t.shape)}")
-    n = len(pages)
-    ints = lambda of: (c_int * n)(*(of(t) for t in pages))
-    return ((c_void_p * n)(*(t.data_ptr() for t in pages)), ints(lambda t: t.shape[0]), ints(lambda t: t.shape[1]), ints(lambda t: t.shape[2]),
-            ints(lambda t: t.shape[4] * t.element_size()))
+        layers, count, heads, _, numbers = t.shape
+        words += (t.data_ptr(), layers, count, heads, numbers * size)
+    return struct.pack(f"{len(words)}q", *words)
 
 
 def copy_pages(pages, src: torch.Tensor, dst: torch.Tensor, rows: Optional[torch.Tensor] = None) -> None:
@@ -2987,11 +3002,11 @@ def copy_pages(pages, src: torch.Tensor, dst: torch.Tensor, rows: Optional[torch
     may be read, or written twice, in the same call; pages that are not there are passed over."""
     lib = _bind()
     pages = list(pages)
-    _on_here("page copies", src, dst, *pages, *(() if rows is None else (rows,)))
+    stream = _on_here("page copies", src, dst, *pages, *(() if rows is None else (rows,)))
     n = src.numel()
     sp, dp = _i32_of(src, n, "source pages"), _i32_of(dst, n, "target pages")
     rp = None if rows is None else _i32_of(rows, n, "copied rows")
-    _check(lib, lib.gi_copy_pages(*_page_tensors(pages, "page copies"), len(pages), sp, dp, rp, n, _stream()), 1 if n and pages else 0)
+    _check(lib, lib.gi_copy_pages(_page_tensors(pages, "page copies"), len(pages), sp, dp, rp, n, stream), 1 if n and pages else 0)
 
 
 def attention_tree(q: torch.Tensor, kcache: torch.Tensor, vcache: torch.Tensor, block_table: torch.Tensor, cu_seqlens: torch.Tensor,
@@ -3003,25 +3018,26 @@ def attention_tree(q: torch.Tensor, kcache: torch.Tensor, vcache: torch.Tensor, 
     32 w + i).  A node that sees nothing gets zeros.  `q`: rows whose first n_heads * head_dim columns are the queries.
     `max_kv_len`: positions and nodes of the longest sequence (sizes the launch; too small a number costs time only)."""
     lib = _bind()
-    _on_here("tree attention", q, kcache, vcache, block_table, cu_seqlens, seq_slots, seq_pos0, masks, out)
+    stream = _on_here("tree attention", q, kcache, vcache, block_table, cu_seqlens, seq_slots, seq_pos0, masks, out)
     _cuda(q, "queries")
     ldq, ldo, dt = _rows(q, "queries"), _rows(out, "attention output"), _dt(q, "queries")
-    if kcache.dtype != q.dtype or vcache.dtype != q.dtype or out.dtype != q.dtype:
+    dtype = q.dtype
+    if kcache.dtype is not dtype or vcache.dtype is not dtype or out.dtype is not dtype:
         raise KernelError("queries, cache and attention output must share a dtype")
     if tuple(kcache.shape[1:]) != (n_kv, 64, head_dim) or kcache.shape != vcache.shape or not kcache.is_contiguous() or not vcache.is_contiguous():
         raise KernelError(f"cache pages must be contiguous [pages, {n_kv}, 64, {head_dim}], got {tuple(kcache.shape)} and {tuple(vcache.shape)}")
-    if n_kv < 1 or n_heads % n_kv or q.shape[1] < n_heads * head_dim or out.shape[0] != q.shape[0] or out.shape[1] < n_heads * head_dim:
+    rows, cols = q.shape
+    if n_kv < 1 or n_heads % n_kv or cols < n_heads * head_dim or out.shape[0] != rows or out.shape[1] < n_heads * head_dim:
         raise KernelError(f"{n_heads} heads over {n_kv} kv heads of {head_dim} do not fit queries {tuple(q.shape)} and output {tuple(out.shape)}")
-    if masks.dim() != 2 or masks.shape[0] != q.shape[0] or masks.dtype != torch.int32 or not masks.is_contiguous():
-        raise KernelError(f"the masks must be contiguous int32 [{q.shape[0]} tokens, words], got {masks.dtype} {tuple(masks.shape)}")
-    if block_table.dim() != 2:
-        raise KernelError("the block table must be [slots, pages]")
+    mp = _i32_rows(masks, "masks")
+    if masks.shape[0] != rows:
+        raise KernelError(f"masks of {masks.shape[0]} tokens for {rows}")
     cu, ss, sp = _i32_of(cu_seqlens, n_seqs + 1, "cu_seqlens"), _i32_of(seq_slots, n_seqs, "slots"), _i32_of(seq_pos0, n_seqs, "start positions")
     nbytes = lib.gi_attn_tree_scratch(n_seqs, max_nodes, max_kv_len, n_heads, n_kv, head_dim, dt)
-    scratch = torch.empty((max(nbytes, 16),), dtype=torch.uint8, device=q.device)
-    _check(lib, lib.gi_attn_tree(out.data_ptr(), ldo, q.data_ptr(), ldq, q.shape[0], dt, kcache.data_ptr(), vcache.data_ptr(), kcache.shape[0],
-                                 _i32(block_table, "block table"), block_table.shape[1], cu, ss, sp, masks.data_ptr(), masks.shape[1], n_seqs, max_nodes,
-                                 max_kv_len, n_heads, n_kv, head_dim, float(scale), scratch.data_ptr(), nbytes, _stream()), 2 if n_seqs else 0)
+    scratch = torch.empty((nbytes,), dtype=torch.uint8, device=q.device)
+    _check(lib, lib.gi_attn_tree(out.data_ptr(), ldo, q.data_ptr(), ldq, rows, dt, kcache.data_ptr(), vcache.data_ptr(), kcache.shape[0],
+                                 _i32_rows(block_table, "block table"), block_table.shape[1], cu, ss, sp, mp, masks.shape[1], n_seqs, max_nodes,
+                                 max_kv_len, n_heads, n_kv, head_dim, scale, scratch.data_ptr(), nbytes, stream), 2 if n_seqs else 0)
     return out
 
 
@@ -3035,17 +3051,17 @@ def tree_commit(picks: torch.Tensor, tokens: torch.Tensor, parents: torch.Tensor
     seq_pos0 + place in the path; a slot of -1 moves nothing."""
     lib = _bind()
     pages = list(pages)
-    _on_here("tree commit", picks, tokens, parents, cu_seqlens, seq_slots, seq_pos0, block_table, *pages)
+    stream = _on_here("tree commit", picks, tokens, parents, cu_seqlens, seq_slots, seq_pos0, block_table, *pages)
     total = picks.numel()
-    pk, tk, pr = (_i32_of(t, total, what) for t, what in ((picks, "picks"), (tokens, "tokens"), (parents, "parents")))
+    pk, tk, pr = _i32_of(picks, total, "picks"), _i32_of(tokens, total, "tokens"), _i32_of(parents, total, "parents")
     cu, ss, sp = _i32_of(cu_seqlens, n_seqs + 1, "cu_seqlens"), _i32_of(seq_slots, n_seqs, "slots"), _i32_of(seq_pos0, n_seqs, "start positions")
     if not 1 <= max_nodes <= MAX_TREE_NODES:
         raise KernelError(f"trees of up to {max_nodes} nodes: 1 to {MAX_TREE_NODES} are supported")
-    if block_table.dim() != 2:
-        raise KernelError("the block table must be [slots, pages]")
-    out = torch.empty((n_seqs * (max_nodes + 2),), dtype=torch.int32, device=picks.device)
-    path, counts, nexts = out[:n_seqs * max_nodes].view(n_seqs, max_nodes), out[n_seqs * max_nodes:n_seqs * (max_nodes + 1)], out[n_seqs * (max_nodes + 1):]
+    device = picks.device
+    path = torch.empty((n_seqs, max_nodes), dtype=torch.int32, device=device)
+    counts = torch.empty((n_seqs,), dtype=torch.int32, device=device)
+    nexts = torch.empty_like(counts)
     _check(lib, lib.gi_tree_commit(path.data_ptr(), counts.data_ptr(), nexts.data_ptr(), pk, tk, pr, cu, ss, sp, n_seqs, max_nodes,
-                                   *_page_tensors(pages, "tree commit"), len(pages), _i32(block_table, "block table"), block_table.shape[1], _stream()),
+                                   _page_tensors(pages, "tree commit"), len(pages), _i32_rows(block_table, "block table"), block_table.shape[1], stream),
            1 if n_seqs else 0)
     return path, counts, nexts
