@@ -3,19 +3,27 @@
 // Beam j of a sequence carries the score s_j (a sum of log probabilities); token v after it is worth
 //     c(j, v) = s_j + x_jv - ln sum_u exp(x_ju)
 // and the `width` largest of a sequence's beams x vocabulary are wanted in order, ties to the lowest j * V + v.  One pass over
-// the logits does both halves: a block holds its stretch of a row in registers, takes the stretch's maximum and sum of
-// exponentials, and lists the stretch's `width` largest logits (within a row the logits' order is the candidates').  A second
-// kernel joins a sequence's stretches: the rows' log sums, then the `width` largest candidates of all lists, compared in 64
-// bits, so that the order between two beams does not hang on the rounding of a sum.
-// What is kept of a stretch must hold its `width` largest, and few more: with the k-th largest of every warp's 32 lane maxima,
-// k = ceil(width / warps), at least `width` logits reach the smallest of the warps' values.  Whatever reaches it goes to a list
-// in shared memory and is put in order by counting.  A list that overflows (rows of equal logits) is made by `width` rounds
-// of a block maximum instead.
-// Bound: the logits' bytes; about ten instructions a logit (one exponential) leave room for them.
+// the logits does both halves: the sum of exponentials, and the `width` largest logits (within a row the logits' order is the
+// candidates').  A second kernel joins a sequence's rows: their log sums, then the `width` largest candidates of all lists,
+// compared in 64 bits, so that the order between two beams does not hang on the rounding of a sum.
+//
+// The rows are cut into tiles of 8,192 logits; a block takes an equal range of the tiles of all rows, so that any number of
+// rows keeps all SMs busy, and leaves one part (sum, list) for every row it meets.  Tiles come through a ring in shared memory
+// (a thread reads back the pieces it asked for itself), which keeps 96 KB an SM under way with few registers; with the next
+// tile in registers instead, the kernel spilled and took twice as long.
+// What enters a part's list must reach a bar that at least `width` of the part's logits reach.  The first bar is the smallest of
+// the warps' k-th largest lane maxima in the part's first tile, k = ceil(width / warps).  After the part's tiles 1, 4, 16, ... the list
+// is cut down to its `width` best and the bar raised to the last of them: each step then adds about 3 `width` entries.  A
+// list that overflows all the same (equal logits) raises the bar and the part is gone through again: entries are ordered by
+// value and then place, no two are alike, and the bar rises every time.
+// A sum that is no number (a logit was none, was infinite, or too large to be scaled) sends the part through once more with every
+// logit looked at: what is no number counts as -inf.
+// Bound: the instructions, about ten a logit (half of them the sum's), next to the logits' bytes.
 #include <math.h>
 
 #include "api.h"
 #include "common.cuh"
+#include "mma_utils.cuh"
 
 namespace {
 
@@ -23,7 +31,8 @@ typedef unsigned long long u64;
 
 constexpr int THREADS = 256, WARPS = THREADS / 32;
 constexpr int MAX_WIDTH = 64, MAX_BEAMS = 64;
-constexpr int CAP = 512;            // entries of a block's list
+constexpr int CAP = 512;                    // entries of a part's list
+constexpr int NUMBERS = 32, STAGES = 2;     // numbers of a tile that a thread takes; tiles of the ring
 
 // Order of floats as order of unsigned numbers; -inf gives the smallest key that occurs.
 __device__ __forceinline__ unsigned order_key(float v) {
@@ -32,26 +41,26 @@ __device__ __forceinline__ unsigned order_key(float v) {
   return (b & 0x80000000u) ? ~b : (b | 0x80000000u);
 }
 __device__ __forceinline__ float key_value(unsigned k) { return __uint_as_float((k & 0x80000000u) ? (k & 0x7fffffffu) : ~k); }
-constexpr unsigned KEY_NONE = 0x007fffffu;    // order_key(-inf)
+__device__ __forceinline__ u64 entry_of(float v, int token) { return ((u64)order_key(v) << 32) | (u64)(~(unsigned)token); }
 
 __device__ __forceinline__ float ex2(float x) {
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
 }
+constexpr float LOG2E = 1.4426950408889634f;
 
-template <typename T> struct Vec;
-template <> struct Vec<float> {
+// A 16-byte piece of a row as it is fetched, and its numbers.
+template <typename T> struct Piece;
+template <> struct Piece<float> {
   static constexpr int N = 4;
-  static __device__ __forceinline__ void load(const float* p, float* x) {
-    const float4 v = __ldcs(reinterpret_cast<const float4*>(p));
-    x[0] = v.x, x[1] = v.y, x[2] = v.z, x[3] = v.w;
+  static __device__ __forceinline__ void numbers(const uint4& v, float* x) {
+    x[0] = __uint_as_float(v.x), x[1] = __uint_as_float(v.y), x[2] = __uint_as_float(v.z), x[3] = __uint_as_float(v.w);
   }
 };
-template <> struct Vec<__nv_bfloat16> {
+template <> struct Piece<__nv_bfloat16> {
   static constexpr int N = 8;
-  static __device__ __forceinline__ void load(const __nv_bfloat16* p, float* x) {
-    const uint4 v = __ldcs(reinterpret_cast<const uint4*>(p));
+  static __device__ __forceinline__ void numbers(const uint4& v, float* x) {
     const unsigned w[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
@@ -61,131 +70,257 @@ template <> struct Vec<__nv_bfloat16> {
   }
 };
 
-// One stretch of one row.  `stretch` numbers (a multiple of a vector); the stretch's aligned middle comes in vectors, the few
-// numbers before and after it one by one (rows of an odd length start on no boundary).
-// part_stat [row][stretches]: (maximum, sum of exponentials above it); part_key [row][stretches][width]: logits in descending
-// order as (order of the value, ~token), 0 where there are no more.
-template <typename T, int VECS>
-__global__ void __launch_bounds__(THREADS, 2)
-beam_stretch_kernel(const T* logits, long ld, int vocab, int stretch, int width, double2* __restrict__ part_stat, u64* __restrict__ part_key) {
-  constexpr int N = Vec<T>::N;
-  __shared__ unsigned s_kth[WARPS];
-  __shared__ float s_max[WARPS];
-  __shared__ double s_sum[WARPS];
-  __shared__ u64 s_list[CAP];
-  __shared__ u64 s_best[WARPS];
-  __shared__ int s_count;
-  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  const int part = blockIdx.x, row = blockIdx.y;
-  if (tid == 0) s_count = 0;
-  gi::pdl_prologue();
+// How the rows are cut, the same on both sides.
+struct Cut {
+  int tiles_row, per, parts;          // tiles of a row, of a block's range; parts of a row that there is room for
+  __host__ __device__ int first_block(int row) const { return (int)((long)row * tiles_row / per); }
+  __host__ __device__ int last_block(int row) const { return (int)(((long)(row + 1) * tiles_row - 1) / per); }
+};
 
-  const T* x_row = logits + (size_t)row * ld;
-  const int lo = part * stretch, hi = min(vocab, lo + stretch);
-  // the first 16-byte boundary at or after the stretch's start, and the last one at or before its end
-  const int lead = (int)((16 - ((uintptr_t)(x_row + lo) & 15)) & 15) / (int)sizeof(T);
-  const int mid_lo = min(hi, lo + lead), vecs = (hi - mid_lo) / N, mid_hi = mid_lo + vecs * N;
-  const int loose = (mid_lo - lo) + (hi - mid_hi);
+// The `width` best of `count` (at most CAP) entries to the front of s_list, in descending order; all threads call it, between two
+// barriers of its own.  Entries that cannot be among them are set aside first by the bar of the first tile's kind.
+struct Lists {
+  u64 list[CAP], passed[CAP];
+  unsigned kth[WARPS];
+  int count, passed_count;
+  u64 bar;
+};
 
-  float x[VECS * N + 1];
-#pragma unroll
-  for (int i = 0; i < VECS; ++i) {
-    const int v = i * THREADS + tid;
-    if (v < vecs) {
-      Vec<T>::load(x_row + mid_lo + v * N, x + i * N);
-    } else {
-#pragma unroll
-      for (int e = 0; e < N; ++e) x[i * N + e] = -INFINITY;
-    }
-  }
-  const int loose_at = tid < mid_lo - lo ? lo + tid : mid_hi + (tid - (mid_lo - lo));
-  x[VECS * N] = tid < loose ? gi::ldf(x_row + loose_at) : -INFINITY;
-  auto token_of = [&](int i) { return i < VECS * N ? mid_lo + ((i / N) * THREADS + tid) * N + i % N : loose_at; };
-
-  float mine = -INFINITY;
-#pragma unroll
-  for (int i = 0; i <= VECS * N; ++i) {
-    x[i] = fmaxf(x[i], -INFINITY);          // what is no number counts as -inf
-    mine = fmaxf(mine, x[i]);
-  }
-  // the k-th largest of the warp's lane maxima
-  const int k = (width + WARPS - 1) / WARPS;
-  unsigned key = order_key(mine), kth = 0, warp_key = 0;
+// The smallest of the warps' k-th largest keys (one a lane): at least k * WARPS keys reach it.
+__device__ __forceinline__ unsigned low_bar(Lists& s, unsigned key, int k) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  unsigned kth = 0;
   for (int r = 0; r < k; ++r) {
     kth = __reduce_max_sync(0xffffffffu, key);
-    if (r == 0) warp_key = kth;
     const unsigned who = __ballot_sync(0xffffffffu, key == kth);
     if (lane == __ffs(who) - 1) key = 0;
   }
-  if (lane == 0) {
-    s_kth[warp] = kth;
-    s_max[warp] = key_value(warp_key);
-  }
+  if (lane == 0) s.kth[warp] = kth;
   __syncthreads();
-  float top = s_max[0];
-  unsigned bar = s_kth[0];
+  unsigned bar = s.kth[0];
 #pragma unroll
-  for (int w = 1; w < WARPS; ++w) {
-    top = fmaxf(top, s_max[w]);
-    bar = min(bar, s_kth[w]);
-  }
-  const float floor_ = key_value(max(bar, KEY_NONE));
-  // the sum of exponentials: in 32 bits over a thread's numbers, in 64 from there on
-  float sum[4] = {0.f, 0.f, 0.f, 0.f};
-  const float base = top > -INFINITY ? top : 0.f;
+  for (int w = 1; w < WARPS; ++w) bar = min(bar, s.kth[w]);
+  return bar;
+}
+
+__device__ __forceinline__ void cut_down(Lists& s, int width) {
+  const int tid = threadIdx.x, count = min(s.count, CAP);
+  if (tid == 0) s.passed_count = 0;
+  u64 own[CAP / THREADS];
 #pragma unroll
-  for (int i = 0; i <= VECS * N; ++i) {
-    sum[i & 3] += ex2((x[i] - base) * 1.4426950408889634f);
-    if (x[i] >= floor_ && x[i] > -INFINITY) {
-      const int at = atomicAdd(&s_count, 1);
-      if (at < CAP) s_list[at] = ((u64)order_key(x[i]) << 32) | (u64)(~(unsigned)token_of(i));
-    }
-  }
-  double total = (double)sum[0] + sum[1] + ((double)sum[2] + sum[3]);
+  for (int q = 0; q < CAP / THREADS; ++q) own[q] = q * THREADS + tid < count ? s.list[q * THREADS + tid] : 0;
+  u64 most = own[0];
 #pragma unroll
-  for (int o = 16; o > 0; o >>= 1) total += __shfl_xor_sync(0xffffffffu, total, o);
-  if (lane == 0) s_sum[warp] = total;
+  for (int q = 1; q < CAP / THREADS; ++q) most = own[q] > most ? own[q] : most;
+  const unsigned bar = low_bar(s, (unsigned)(most >> 32), (width + WARPS - 1) / WARPS);
+#pragma unroll
+  for (int q = 0; q < CAP / THREADS; ++q)
+    if (own[q] != 0 && (unsigned)(own[q] >> 32) >= bar) s.passed[atomicAdd(&s.passed_count, 1)] = own[q];
   __syncthreads();
-  const size_t at_part = (size_t)row * gridDim.x + part;
-  if (tid == 0) {
-    double t = 0.0;
-    for (int w = 0; w < WARPS; ++w) t += s_sum[w];
-    part_stat[at_part] = make_double2((double)top, t);
+  const int passed = s.passed_count;
+  for (int i = tid; i < passed; i += THREADS) {
+    const u64 mine = s.passed[i];
+    int place = 0;
+    for (int o = 0; o < passed; ++o) place += s.passed[o] > mine ? 1 : 0;
+    if (place < width) s.list[place] = mine;
+    if (place == width - 1) s.bar = mine;
   }
-  u64* out = part_key + at_part * width;
-  const int count = s_count;
-  if (count <= CAP) {
-    for (int i = tid; i < count; i += THREADS) {
-      const u64 own = s_list[i];
-      int place = 0;
-      for (int o = 0; o < count; ++o) place += s_list[o] > own ? 1 : 0;      // no two are alike
-      if (place < width) out[place] = own;
+  if (tid == 0) s.count = min(count, width);
+  __syncthreads();
+}
+
+// part_stat [row][parts]: (reference in powers of two, sum of 2^(x log2 e - reference)); part_key [row][parts][width]: logits in descending order as
+// (order of the value, ~token), 0 where there are no more.
+template <typename T>
+__global__ void __launch_bounds__(THREADS, 3)
+beam_rows_kernel(const T* logits, long ld, int vocab, int rows, Cut cut, int width, double2* __restrict__ part_stat, u64* __restrict__ part_key) {
+  constexpr int N = Piece<T>::N, VPT = NUMBERS / N;
+  extern __shared__ __align__(16) unsigned char smem[];
+  uint4* ring = (uint4*)smem;                        // [STAGES][VPT][THREADS]
+  __shared__ Lists s;
+  __shared__ float s_ref[WARPS];
+  __shared__ double s_sum[WARPS];
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  gi::pdl_prologue();
+  const long lo = (long)blockIdx.x * cut.per, hi = min((long)rows * cut.tiles_row, lo + cut.per);
+
+  // A row's 16-byte pieces lie between the first 16-byte boundary in it and the last; the few numbers before and after them go
+  // with its first tile.
+  struct Row {
+    const T* x;
+    int lead, pieces, tail;
+  };
+  auto row_of = [&](int row) {
+    Row r;
+    r.x = logits + (size_t)row * ld;
+    r.lead = min(vocab, (int)((16 - ((uintptr_t)r.x & 15)) & 15) / (int)sizeof(T));
+    r.pieces = (vocab - r.lead) / N;
+    r.tail = vocab - r.lead - r.pieces * N;
+    return r;
+  };
+  // a place in the list of tiles, counted up without divisions
+  struct Place {
+    int left, row, tile, stage;                      // tiles up to the end of the block's range
+    __device__ __forceinline__ void next(int tiles_row) {
+      --left;
+      if (++tile == tiles_row) tile = 0, ++row;
+      if (++stage == STAGES) stage = 0;
     }
-    for (int i = count + tid; i < width; i += THREADS) out[i] = 0;
-    return;
-  }
-  u64 last = ~(u64)0;
-  for (int r = 0; r < width; ++r) {
-    u64 best = 0;
+  };
+  Place here;
+  here.left = (int)max(0L, hi - lo), here.row = (int)(lo / cut.tiles_row), here.tile = (int)(lo - (long)here.row * cut.tiles_row), here.stage = 0;
+  Place asked = here;                                // the next tile to ask for
+  auto ask = [&]() {
+    if (asked.left > 0) {
+      const Row r = row_of(asked.row);
+      const uint4* body = reinterpret_cast<const uint4*>(r.x + r.lead);
+      uint4* to = ring + asked.stage * VPT * THREADS + tid;
 #pragma unroll
-    for (int i = 0; i <= VECS * N; ++i) {
-      const u64 own = x[i] > -INFINITY ? ((u64)order_key(x[i]) << 32) | (u64)(~(unsigned)token_of(i)) : 0;
-      if (own < last && own > best) best = own;
+      for (int i = 0; i < VPT; ++i) {
+        const int at = (asked.tile * VPT + i) * THREADS + tid;
+        if (at < r.pieces) gi::cp_async_16(gi::smem_u32(to + i * THREADS), body + at, 16);
+      }
     }
+    asked.next(cut.tiles_row);
+    gi::cp_async_commit();
+  };
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) {
-      const u64 other = __shfl_xor_sync(0xffffffffu, best, o);
-      best = other > best ? other : best;
+  for (int i = 0; i < STAGES - 1; ++i) ask();
+
+  Place part = here;                                 // the part's first tile
+  int summed = here.left;                            // the sums hold every tile with more than that many left
+  int next_cut = 1;                                  // tiles of the part after which its list is cut down
+  float ref = 0.f, sum = 0.f;                        // of this thread's numbers: sum of 2^(x log2 e - ref)
+  bool keep_bar = false, careful = false;            // a part that is gone through again, and what for
+  while (here.left > 0) {
+    const int row = here.row, tile = here.tile;
+    const Row r = row_of(row);
+    ask();
+    gi::cp_async_wait<STAGES - 1>();
+    float x[VPT * N + 1];
+    const uint4* from = ring + here.stage * VPT * THREADS + tid;
+#pragma unroll
+    for (int i = 0; i < VPT; ++i) Piece<T>::numbers(from[i * THREADS], x + i * N);
+    if ((tile + 1) * VPT * THREADS > r.pieces) {
+#pragma unroll
+      for (int i = 0; i < VPT; ++i)
+        if ((tile * VPT + i) * THREADS + tid >= r.pieces) {
+#pragma unroll
+          for (int e = 0; e < N; ++e) x[i * N + e] = -INFINITY;
+        }
     }
-    if (lane == 0) s_best[warp] = best;
+    const int loose_at = tid < r.lead ? tid : vocab - r.tail + (tid - r.lead);
+    x[NUMBERS] = tile == 0 && tid < r.lead + r.tail ? gi::ldf(r.x + loose_at) : -INFINITY;
+    if (__builtin_expect(careful, false)) {
+#pragma unroll
+      for (int i = 0; i <= NUMBERS; ++i) x[i] = fmaxf(x[i], -INFINITY);
+    }
+    float tops[2] = {x[NUMBERS], -INFINITY};           // (a maximum passes over what is no number)
+#pragma unroll
+    for (int i = 0; i < NUMBERS; ++i) tops[i & 1] = fmaxf(tops[i & 1], x[i]);
+    const float mine = fmaxf(fmaxf(tops[0], tops[1]), -INFINITY);
+
+    const bool first = here.left == part.left;
+    if (first) {
+      unsigned bar = 0;
+      if (!keep_bar) bar = low_bar(s, order_key(mine), (width + WARPS - 1) / WARPS);
+      if (tid == 0) {
+        s.count = 0;
+        if (!keep_bar) s.bar = (u64)bar << 32;
+      }
+      next_cut = 1;
+      if (summed == here.left) ref = 0.f, sum = 0.f;
+      __syncthreads();
+    }
+    if (summed == here.left) {
+      // a thread's reference moves up with its maximum
+      if (mine > -INFINITY) {
+        // (scaled, unless it is too large for that: those parts are gone through carefully, with the reference itself)
+        const float top = careful ? mine : mine * LOG2E;
+        if (top > ref || sum == 0.f) {
+          sum = sum == 0.f ? 0.f : sum * ex2(careful ? (ref - top) * LOG2E : ref - top);
+          ref = top;
+        }
+        float more[4] = {0.f, 0.f, 0.f, 0.f};
+        if (__builtin_expect(careful, false)) {
+#pragma unroll
+          for (int i = 0; i <= NUMBERS; ++i) more[i & 3] += ex2((x[i] - ref) * LOG2E);
+        } else {
+#pragma unroll
+          for (int i = 0; i <= NUMBERS; ++i) more[i & 3] += ex2(fmaf(x[i], LOG2E, -ref));
+        }
+        sum += (more[0] + more[1]) + (more[2] + more[3]);
+      }
+      --summed;
+    }
+    const u64 bar = s.bar;
+    const float bar_value = fmaxf(key_value((unsigned)(bar >> 32)), -3.402823466e38f);      // (-inf is nobody's candidate)
+    if (mine >= bar_value) {
+      // which of the thread's numbers reach it, and one after the other from where they lie (33 copies of what follows, one for every
+      // register, took more time to fetch than to execute)
+      u64 hits = 0;
+#pragma unroll
+      for (int i = 0; i <= NUMBERS; ++i) hits |= x[i] >= bar_value ? (u64)1 << i : 0;
+      while (hits != 0) {
+        const int i = __ffsll((long long)hits) - 1;
+        hits &= hits - 1;
+        const float v = i < NUMBERS ? gi::ldf(reinterpret_cast<const T*>(from + i / N * THREADS) + i % N) : gi::ldf(r.x + loose_at);
+        const u64 own = entry_of(v, i < NUMBERS ? r.lead + ((tile * VPT + i / N) * THREADS + tid) * N + i % N : loose_at);
+        if (own >= bar) {
+          const int to = atomicAdd(&s.count, 1);
+          if (to < CAP) s.list[to] = own;
+        }
+      }
+    }
+    const bool last = tile + 1 == cut.tiles_row || here.left == 1;
+    here.next(cut.tiles_row);
+    if (!last && part.left - here.left < next_cut) continue;
+    next_cut *= 4;
     __syncthreads();
-    best = s_best[0];
+    const bool over = s.count > CAP;
+    cut_down(s, width);
+    if (over) {
+      // the bar is the `width`-th best of what the list had room for: once more from the part's first tile
+      gi::cp_async_wait<0>();
+      here = asked = part;
 #pragma unroll
-    for (int w = 1; w < WARPS; ++w) best = s_best[w] > best ? s_best[w] : best;
+      for (int i = 0; i < STAGES - 1; ++i) ask();
+      keep_bar = true;
+      continue;
+    }
+    if (!last) continue;
+    // the part's sum, in 64 bits over the threads, above the largest reference
+    const float own_ref = sum != 0.f ? ref : -INFINITY;
+    float top_ref = gi::warp_max(own_ref);
+    if (lane == 0) s_ref[warp] = top_ref;
+    const bool none = __syncthreads_or(!(fabsf(sum) < INFINITY) || (sum != 0.f && !(fabsf(ref) < INFINITY)));
+    if (none && !careful) {
+      careful = keep_bar = true;                       // (the bar that the list ended with is reached by `width` logits)
+      summed = part.left;
+      gi::cp_async_wait<0>();
+      here = asked = part;
+#pragma unroll
+      for (int i = 0; i < STAGES - 1; ++i) ask();
+      continue;
+    }
+#pragma unroll
+    for (int w = 0; w < WARPS; ++w) top_ref = fmaxf(top_ref, s_ref[w]);
+    double total = sum != 0.f ? (double)sum * (double)ex2(careful ? (own_ref - top_ref) * LOG2E : own_ref - top_ref) : 0.0;
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) total += __shfl_xor_sync(0xffffffffu, total, o);
+    if (lane == 0) s_sum[warp] = total;
+    const size_t out = (size_t)row * cut.parts + (blockIdx.x - cut.first_block(row));
+    for (int i = tid; i < width; i += THREADS) part_key[out * width + i] = i < s.count ? s.list[i] : 0;
     __syncthreads();
-    if (tid == 0) out[r] = best;
-    last = best;
+    if (tid == 0) {
+      double t = 0.0;
+      for (int w = 0; w < WARPS; ++w) t += s_sum[w];
+      part_stat[out] = make_double2(careful ? (double)top_ref * 1.4426950408889634 : (double)top_ref, t);
+    }
+    keep_bar = careful = false;
+    part = here;
   }
+  gi::cp_async_wait<0>();
 }
 
 // A candidate of the join: worth more, or as much and earlier among beams x vocabulary.
@@ -195,81 +330,121 @@ struct Candidate {
   __device__ __forceinline__ bool before(const Candidate& o) const { return c > o.c || (c == o.c && at < o.at); }
 };
 
-// One block joins a sequence's lists (`beams` x `parts`, each in descending order).
+// Order of doubles as order of unsigned numbers.
+__device__ __forceinline__ u64 order_key(double v) {
+  const u64 b = (u64)__double_as_longlong(v + 0.0);
+  return (b >> 63) ? ~b : (b | 0x8000000000000000ull);
+}
+
+// One block joins a sequence's lists (those of the parts of its rows).  Every candidate is looked at twice, by all threads side by
+// side: for a bar that `width` of them reach (as in the rows' first tiles, on the upper halves of the candidates' keys), and for
+// those that reach it, which are put in order by counting.
 __global__ void __launch_bounds__(THREADS)
-beam_join_kernel(const float* scores, const double2* part_stat, const u64* part_key, int beams, int parts, int width, int vocab,
+beam_join_kernel(const float* scores, const double2* part_stat, const u64* part_key, int beams, Cut cut, int width, int vocab,
                  float* __restrict__ out_scores, int* __restrict__ out_parents, int* __restrict__ out_tokens) {
-  extern __shared__ double s_base[];              // [beams], then every list's first candidate [beams * parts]
-  __shared__ Candidate s_list[CAP];
+  constexpr int AHEAD = 4;
+  __shared__ double s_base[MAX_BEAMS];
+  __shared__ int s_parts[MAX_BEAMS];              // parts that a row has
+  __shared__ Lists s;
+  __shared__ Candidate s_passed[CAP];
   __shared__ Candidate s_best[WARPS];
-  __shared__ int s_count;
-  __shared__ double s_floor;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  const int seq = blockIdx.x, lists = beams * parts;
-  double* s_head = s_base + beams;
-  if (tid == 0) {
-    s_count = 0;
-    s_floor = -INFINITY;
-  }
+  const int seq = blockIdx.x, parts = cut.parts, entries = beams * parts * width;
+  if (tid < beams) s_parts[tid] = cut.last_block(seq * beams + tid) - cut.first_block(seq * beams + tid) + 1;
+  if (tid == 0) s.passed_count = 0;
+  __syncthreads();
   gi::pdl_prologue();
-  // a row's log sum, its stretches in order
-  for (int j = tid; j < beams; j += THREADS) {
-    const double2* st = part_stat + (size_t)(seq * beams + j) * parts;
-    double top = -INFINITY;
-    for (int p = 0; p < parts; ++p) top = fmax(top, st[p].x);
-    double sum = 0.0;
-    if (top > -INFINITY)
-      for (int p = 0; p < parts; ++p) sum += st[p].y * exp(st[p].x - top);
-    const double base = (double)scores[(size_t)seq * beams + j] - (top + log(sum));
-    s_base[j] = isfinite(base) ? base : -INFINITY;      // nothing but -inf, or a logit that is +inf: the beam offers nothing
-  }
-  __syncthreads();
-  const u64* keys = part_key + (size_t)seq * lists * width;
-  auto candidate = [&](int list, int i) {
-    const u64 key = keys[(size_t)list * width + i];
-    Candidate out;
-    const double base = s_base[list / parts];
-    out.c = key == 0 || !(base > -INFINITY) ? -INFINITY : base + (double)key_value((unsigned)(key >> 32));
-    out.at = (long)(list / parts) * vocab + (long)(~(unsigned)(key & 0xffffffffu));
-    return out;
+  const u64* keys = part_key + (size_t)seq * entries;
+  // the first entries' keys are under way while the rows' sums are made; parts that a row does not have count as empty
+  auto key_at = [&](int e, int& j) {
+    const int list = min(e, entries - 1) / width;
+    j = list / parts;
+    return e < entries && list - j * parts < s_parts[j] ? keys[e] : 0;
   };
-  // a floor that at least `width` candidates reach: the `width`-th largest of the lists' first ones, or, with fewer lists than
-  // that, the smallest of the lists' k-th ones
-  const int k = (width + lists - 1) / lists;
-  for (int l = tid; l < lists; l += THREADS) s_head[l] = candidate(l, k - 1).c;
-  __syncthreads();
-  const int wanted = min(width, lists) - 1;
-  for (int l = tid; l < lists; l += THREADS) {
-    const double own = s_head[l];
-    int place = 0;
-    for (int o = 0; o < lists; ++o) place += (s_head[o] > own || (s_head[o] == own && o < l)) ? 1 : 0;
-    if (place == wanted) s_floor = own;
+  // Neighbouring entries go to different warps, in another order from list to list: a warp that had the lists of one bad beam
+  // alone, or the lists' ends alone, would hold the bar down.
+  auto place_of = [&](int q) {
+    const int e0 = q * THREADS + lane * WARPS;
+    return e0 + ((warp + e0 / width) & (WARPS - 1));
+  };
+  u64 ahead[AHEAD];
+  int beam_ahead[AHEAD];
+#pragma unroll
+  for (int q = 0; q < AHEAD; ++q) {
+    beam_ahead[q] = 0;
+    const int e = place_of(q);
+    ahead[q] = e < entries ? key_at(e, beam_ahead[q]) : 0;
+  }
+  // a row's log sum: a warp to a row, a lane to a part
+  for (int j = warp; j < beams; j += WARPS) {
+    const double2* st = part_stat + ((size_t)seq * beams + j) * parts;
+    const double score = (double)scores[(size_t)seq * beams + j];
+    double top = -INFINITY, sum = 0.0;
+    for (int p = lane; p < s_parts[j]; p += 32) {
+      const double2 v = st[p];
+      const double both = fmax(top, v.x);
+      if (both > -INFINITY) sum = (top > -INFINITY ? sum * exp2(top - both) : 0.0) + (v.x > -INFINITY ? v.y * exp2(v.x - both) : v.y);
+      top = both;
+    }
+    double both = top;
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) both = fmax(both, __shfl_xor_sync(0xffffffffu, both, o));
+    sum = top > -INFINITY ? sum * exp2(top - both) : sum;
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+    const double base = score - (both * 0.69314718055994530942 + log(sum));
+    if (lane == 0) s_base[j] = isfinite(base) ? base : -INFINITY;      // nothing but -inf, or a logit that is +inf: the beam offers nothing
   }
   __syncthreads();
-  const double floor_ = s_floor;
-  for (int l = tid; l < lists; l += THREADS)
-    for (int i = 0; i < width; ++i) {
-      const Candidate own = candidate(l, i);
-      if (!(own.c >= floor_) || !(own.c > -INFINITY)) break;
-      const int at = atomicAdd(&s_count, 1);
-      if (at < CAP) s_list[at] = own;
-    }
+  auto candidate = [&](u64 key, int j) {
+    const double base = s_base[j];
+    Candidate own;
+    own.c = key == 0 || !(base > -INFINITY) ? -INFINITY : base + (double)key_value((unsigned)(key >> 32));
+    own.at = (long)j * vocab + (long)(~(unsigned)(key & 0xffffffffu));
+    return own;
+  };
+  auto entry = [&](int q, int e) {                  // the q-th of this thread's entries
+    if (q < AHEAD) return candidate(ahead[q & (AHEAD - 1)], beam_ahead[q & (AHEAD - 1)]);
+    int j;
+    const u64 key = key_at(e, j);
+    return candidate(key, j);
+  };
+  unsigned most = 0;
+#pragma unroll
+  for (int q = 0; q < AHEAD; ++q) {
+    const double c = entry(q, 0).c;
+    if (c > -INFINITY) most = max(most, (unsigned)(order_key(c) >> 32));
+  }
+  for (int q = AHEAD; q * THREADS < entries; ++q) {
+    const double c = entry(AHEAD, place_of(q)).c;
+    if (c > -INFINITY) most = max(most, (unsigned)(order_key(c) >> 32));
+  }
+  const unsigned bar = low_bar(s, most, (width + WARPS - 1) / WARPS);
+  auto pass = [&](const Candidate& own) {
+    if (!(own.c > -INFINITY) || (unsigned)(order_key(own.c) >> 32) < bar) return;
+    const int at = atomicAdd(&s.passed_count, 1);
+    if (at < CAP) s_passed[at] = own;
+  };
+#pragma unroll
+  for (int q = 0; q < AHEAD; ++q) pass(entry(q, 0));
+  for (int q = AHEAD; q * THREADS < entries; ++q) pass(entry(AHEAD, place_of(q)));
   __syncthreads();
-  const int count = s_count;
+  const int count = s.passed_count;
   auto store = [&](int place, const Candidate& own) {
     const size_t o = (size_t)seq * width + place;
     const bool none = !(own.c > -INFINITY);
+    const int parent = none ? -1 : (int)(own.at / vocab);
     out_scores[o] = (float)own.c;
-    out_parents[o] = none ? -1 : (int)(own.at / vocab);
-    out_tokens[o] = none ? -1 : (int)(own.at % vocab);
+    out_parents[o] = parent;
+    out_tokens[o] = none ? -1 : (int)(own.at - (long)parent * vocab);
   };
   Candidate none;
   none.c = -INFINITY, none.at = 0;
   if (count <= CAP) {
     for (int i = tid; i < count; i += THREADS) {
-      const Candidate own = s_list[i];
+      const Candidate own = s_passed[i];
       int place = 0;
-      for (int o = 0; o < count; ++o) place += s_list[o].before(own) ? 1 : 0;
+      for (int o = 0; o < count; ++o) place += s_passed[o].before(own) ? 1 : 0;
       if (place < width) store(place, own);
     }
     for (int i = count + tid; i < width; i += THREADS) store(i, none);
@@ -280,15 +455,10 @@ beam_join_kernel(const float* scores, const double2* part_stat, const u64* part_
   for (int r = 0; r < width; ++r) {
     Candidate best = none;
     best.at = 0x7fffffffffffffffL;
-    for (int l = tid; l < lists; l += THREADS)
-      for (int i = 0; i < width; ++i) {
-        const Candidate own = candidate(l, i);
-        if (!(own.c > -INFINITY)) break;
-        if (last.before(own)) {
-          if (own.before(best)) best = own;
-          break;                                    // a list is in descending order: what follows is worth less
-        }
-      }
+    for (int e = tid; e < entries; e += THREADS) {
+      const Candidate own = entry(AHEAD, e);
+      if (own.c > -INFINITY && last.before(own) && own.before(best)) best = own;
+    }
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) {
       Candidate other;
@@ -307,31 +477,42 @@ beam_join_kernel(const float* scores, const double2* part_stat, const u64* part_
   }
 }
 
-// How a row is cut: stretches that a block's registers hold, more of them while the launch would leave SMs without a block.
-int beam_parts(int rows, int vocab) {
-  constexpr int MOST = THREADS * 64;
-  int parts = (vocab + MOST - 1) / MOST;
-  const int want = (2 * gi::sm_count() + rows - 1) / rows;
-  const int fine = (vocab + THREADS * 16 - 1) / (THREADS * 16);
-  return parts < want ? (want < fine ? (want > parts ? want : parts) : (fine > parts ? fine : parts)) : parts;
+struct Plan {
+  Cut cut;
+  int blocks;
+};
+
+template <typename T> constexpr int SMEM_RING = STAGES * THREADS * NUMBERS * (int)sizeof(T);
+
+Plan plan_of(int rows, int vocab) {
+  const int tile = THREADS * NUMBERS;
+  Plan p;
+  p.cut.tiles_row = (vocab + tile - 1) / tile;
+  const long slots = 3L * gi::sm_count(), total = (long)rows * p.cut.tiles_row;
+  p.cut.per = (int)((total + slots - 1) / slots);
+  p.blocks = (int)((total + p.cut.per - 1) / p.cut.per);
+  p.cut.parts = (p.cut.tiles_row + p.cut.per - 2) / p.cut.per + 1;
+  return p;
 }
 
 template <typename T>
-int launch_beam(const T* logits, long ld, int rows, int vocab, int parts, int width, double2* stat, u64* key, cudaStream_t s) {
-  constexpr int N = Vec<T>::N;
-  // stretches of whole vectors; the loose numbers at both ends of an unaligned one have a register of their own
-  const int stretch = ((vocab + parts - 1) / parts + N - 1) / N * N;
-  const dim3 grid(parts, rows);
-  if (stretch <= THREADS * 16)
-    return gi::check(gi::launch(beam_stretch_kernel<T, 16 / N>, grid, dim3(THREADS), 0, s, logits, ld, vocab, stretch, width, stat, key), "beam selection");
-  return gi::check(gi::launch(beam_stretch_kernel<T, 64 / N>, grid, dim3(THREADS), 0, s, logits, ld, vocab, stretch, width, stat, key), "beam selection");
+int launch_rows(const T* logits, long ld, int vocab, int rows, const Plan& p, int width, double2* stat, u64* key, cudaStream_t s) {
+  auto kern = beam_rows_kernel<T>;
+  static bool configured[gi::MAX_DEVICES_SEEN] = {false};
+  int dev;
+  if (gi::unconfigured_here(configured, &dev)) {
+    cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM_RING<T>);
+    if (e != cudaSuccess) return gi::fail(GI_ERR_CUDA, "beam selection: %s", cudaGetErrorString(e));
+    if (dev >= 0) configured[dev] = true;
+  }
+  return gi::check(gi::launch(kern, dim3(p.blocks), dim3(THREADS), SMEM_RING<T>, s, logits, ld, vocab, rows, p.cut, width, stat, key), "beam selection");
 }
 
 }  // namespace
 
 extern "C" long gi_beam_select_scratch(int rows, int vocab, int width) {
   if (rows <= 0 || vocab <= 0 || width <= 0) return 0;
-  return (long)rows * beam_parts(rows, vocab) * (16 + 8L * width);
+  return (long)rows * plan_of(rows, vocab).cut.parts * (16 + 8L * width);
 }
 
 extern "C" int gi_beam_select(float* out_scores, int* out_parents, int* out_tokens, const void* logits, int dtype, long ld, const float* scores,
@@ -341,18 +522,19 @@ extern "C" int gi_beam_select(float* out_scores, int* out_parents, int* out_toke
   if (vocab < 1 || ld < vocab) return gi::fail(GI_ERR_ARG, "beam selection: rows of %d logits at a stride of %ld", vocab, ld);
   if (width < 1 || width > MAX_WIDTH || (long)width > (long)beams * vocab)
     return gi::fail(GI_ERR_ARG, "beam selection: a width of %d, 1 to %d (and at most beams x vocabulary) are supported", width, MAX_WIDTH);
-  if ((long)seqs * beams > 65535) return gi::fail(GI_ERR_UNSUPPORTED, "beam selection: more than 65535 rows in one launch");
-  const int rows = seqs * beams, parts = beam_parts(rows, vocab);
+  if ((long)seqs * beams > 0x3fffffL || vocab > 0x3fffffff) return gi::fail(GI_ERR_UNSUPPORTED, "beam selection: %ld rows of %d logits in one launch", (long)seqs * beams, vocab);
+  if (dtype != GI_F32 && dtype != GI_BF16) return gi::fail(GI_ERR_ARG, "beam selection: unknown dtype code %d", dtype);
+  const int rows = seqs * beams;
+  const Plan p = plan_of(rows, vocab);
   if (scratch_bytes < gi_beam_select_scratch(rows, vocab, width) || ((uintptr_t)scratch & 15))
     return gi::fail(GI_ERR_ARG, "beam selection: the scratch memory is too small or not aligned");
+  if ((long)beams * p.cut.parts * width > 0x3fffffffL) return gi::fail(GI_ERR_UNSUPPORTED, "beam selection: %d beams in %d parts each", beams, p.cut.parts);
   double2* stat = (double2*)scratch;
-  u64* key = (u64*)(stat + (size_t)rows * parts);
+  u64* key = (u64*)(stat + (size_t)rows * p.cut.parts);
   cudaStream_t s = (cudaStream_t)stream;
   int rc = GI_OK;
-  GI_DISPATCH_DTYPE(dtype, T, rc = launch_beam((const T*)logits, ld, rows, vocab, parts, width, stat, key, s));
+  GI_DISPATCH_DTYPE(dtype, T, rc = launch_rows((const T*)logits, ld, vocab, rows, p, width, stat, key, s));
   if (rc != GI_OK) return rc;
-  const size_t smem = (size_t)(beams + beams * parts) * sizeof(double);
-  if (smem > 36 * 1024) return gi::fail(GI_ERR_UNSUPPORTED, "beam selection: %d beams over %d stretches", beams, parts);
-  return gi::check(gi::launch(beam_join_kernel, dim3(seqs), dim3(THREADS), smem, s, scores, stat, key, beams, parts, width, vocab, out_scores,
+  return gi::check(gi::launch(beam_join_kernel, dim3(seqs), dim3(THREADS), 0, s, scores, stat, key, beams, p.cut, width, vocab, out_scores,
                               out_parents, out_tokens), "beam selection (join)");
 }
