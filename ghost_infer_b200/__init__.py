@@ -28,10 +28,10 @@ from .config.sofopel import SofopelConfig, build_sofopel_spec
 
 register_architecture("Sofopel", SofopelConfig.from_dict, build_sofopel_spec, replace=True)
 
-from .engine import Engine, Model, StepEntry  # noqa: E402
+from .engine import Engine, Model, StepEntry, TreeEntry  # noqa: E402
 from .api import LLM  # noqa: E402
 from .sampling import SamplingParams  # noqa: E402
 
 __all__ = ["ConfigError", "LlamaConfig", "BarovikConfig", "NavalornConfig", "NuzinexConfig", "TorutarConfig", "VavupelConfig", "SofopelConfig", "UnknownArchitectureError", "load_config", "register_architecture",
-           "registered_architectures", "Engine", "Model", "StepEntry", "LLM", "SamplingParams"]
+           "registered_architectures", "Engine", "Model", "StepEntry", "TreeEntry", "LLM", "SamplingParams"]
 __version__ = "0.1.0"

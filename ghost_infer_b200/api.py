@@ -12,6 +12,8 @@ from __future__ import annotations
 
 from typing import List, Mapping, Optional, Sequence
 
+from .engine.beams import BeamResult, BeamSearch
+from .engine.drafted import DraftedLoop, PromptLookup
 from .engine.generate import GenerationLoop, GenerationResult, GenerationStats
 from .engine.model import Model
 from .engine.step import Engine
@@ -55,7 +57,33 @@ class LLM:
                               max_step_tokens=max_step_tokens, time_steps_every=time_steps_every)
         results = loop.run(prompts, max_new)
         self.last_stats = loop.stats
+        self._check_kernels()
+        return results
+
+    def _check_kernels(self) -> None:
         if self.model.rt.device.type == "cuda":
             from .kernels import ops
             ops.check_status()          # a kernel whose bounded wait ran out has said so: never hand out its tokens silently
+
+    def beam_search(self, prompts: Sequence[Sequence[int]], beams: int = 4, max_new: int = 256, length_penalty: float = 1.0,
+                    stop_token_ids: Optional[Sequence[int]] = None, batch_size: int = 1) -> List[List[BeamResult]]:
+        """The `beams` (1 to 32) best continuations of every prompt that beam search finds, best first, `batch_size` prompts at a
+        time.  Results are ordered by log probability / tokens ** length_penalty; a search ends when as many results have
+        ended as there are beams and nothing still going is more probable, or at `max_new` tokens."""
+        stop = self.stop_token_ids if stop_token_ids is None else stop_token_ids
+        out = BeamSearch(self.engine, beams, stop, length_penalty, batch_size).run(prompts, max_new)
+        self._check_kernels()
+        return out
+
+    def generate_drafted(self, prompts: Sequence[Sequence[int]], max_new: int = 256, drafter=None, max_nodes: int = 32,
+                         stop_token_ids: Optional[Sequence[int]] = None, batch_size: int = 8) -> List[GenerationResult]:
+        """`generate` at temperature 0, several tokens a step where a draft is right.  `drafter(tokens, most)` gives at most `most`
+        tokens that may follow and, for each, which of them it continues (-1: the last of `tokens`); None: `PromptLookup`, what
+        followed the same words earlier in the sequence.  `max_nodes` (1 to 256): tokens a sequence runs in one step.  For models
+        that attend to all cached positions in every layer."""
+        stop = self.stop_token_ids if stop_token_ids is None else stop_token_ids
+        loop = DraftedLoop(self.engine, drafter if drafter is not None else PromptLookup(), stop, batch_size, max_nodes)
+        results = loop.run(prompts, max_new)
+        self.last_stats = loop.stats
+        self._check_kernels()
         return results

@@ -6,7 +6,8 @@ layer, src/cuda.rs:9945-9975), and rewinds by lowering `pos` (src/model.rs:803-8
 A batch needs the same per sequence, so the unit here is a slot: one sequence's
 length and its list of pages.  Pages are `PAGE_TOKENS` positions wide; a pool
 hands them out and takes them back, so memory is sized by the tokens that are
-alive, not by slots x longest sequence.  Lengths are the only truth: rows past
+alive, not by slots x longest sequence.  Sequences that continue the same one
+(beams) hold its pages together: a page goes back when its last holder lets go.  Lengths are the only truth: rows past
 a slot's length are never read, so a page needs no clearing when it is reused.
 """
 from __future__ import annotations
@@ -35,7 +36,7 @@ class PagePool:
             raise ValueError("a pool needs at least one usable page")
         self.n_pages = n_pages            # usable pages, numbered 1..n_pages
         self._free: List[int] = list(range(n_pages, 0, -1))
-        self._held = [False] * (n_pages + 1)
+        self._holders = [0] * (n_pages + 1)
 
     @property
     def free_pages(self) -> int:
@@ -46,15 +47,26 @@ class PagePool:
             raise CacheFullError(f"the cache is full: {n} more pages wanted, {len(self._free)} of {self.n_pages} free")
         out = [self._free.pop() for _ in range(n)]
         for p in out:
-            self._held[p] = True
+            self._holders[p] = 1
         return out
+
+    def holders(self, page: int) -> int:
+        return self._holders[page]
+
+    def share(self, pages: Sequence[int]) -> None:
+        """One more holder for each of these pages."""
+        for p in pages:
+            if p <= 0 or p > self.n_pages or not self._holders[p]:
+                raise RuntimeError(f"page {p} is shared but not held")
+            self._holders[p] += 1
 
     def give_back(self, pages: Sequence[int]) -> None:
         for p in pages:
-            if p <= 0 or p > self.n_pages or not self._held[p]:
+            if p <= 0 or p > self.n_pages or not self._holders[p]:
                 raise RuntimeError(f"page {p} is given back but not held")
-            self._held[p] = False
-            self._free.append(p)
+            self._holders[p] -= 1
+            if not self._holders[p]:
+                self._free.append(p)
 
 
 class SlotAllocator:

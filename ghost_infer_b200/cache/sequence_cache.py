@@ -14,6 +14,9 @@ Storage of a group: K and V, each `[entry, page, kv_head, PAGE_TOKENS, head_dim]
 place of `head_dim` where a mixer's values are not as wide as its keys).  One page of one kv head is a
 contiguous block, which is what the decode kernel streams.
 
+Several slots may continue the same sequence (`fork`, `reorder`): they hold its pages together, and a slot gets a page of its
+own, with a copy of what is filled of it, when it is about to write to one that others hold (`reserve`).
+
 Kinds of request: "full" keeps every position; "window" only the last `window` positions; "chunk" only the
 positions of the chunk of `window` positions (counted from position 0) that the sequence's newest token lies in.
 The last two give pages back as the sequence moves on.
@@ -204,7 +207,8 @@ class SequenceCache:
         return self.lengths[slot]
 
     def reserve(self, wanted: Sequence[Tuple[int, int]]) -> None:
-        """Pages for every (slot, new length) pair, in every group; all or nothing."""
+        """Pages for every (slot, new length) pair, in every group; all or nothing.  What will be written, from a slot's
+        length on, lies in pages that the slot holds alone afterwards: the one its last tokens share with others is copied."""
         for slot, new_len in wanted:
             if not self.slots.live(slot):
                 raise RuntimeError(f"slot {slot} is not open")
@@ -212,6 +216,12 @@ class SequenceCache:
                 raise CacheFullError(f"context full ({self.max_seq_len} tokens): slot {slot} would hold {new_len}")
         for g in self._groups:
             need = sum(max(0, pages_for(n) - len(g.pages[s])) for s, n in wanted)
+            shared: Dict[int, int] = {}                     # page held by others too -> how many of `wanted` want it for themselves
+            for s, n in wanted:
+                for page in self._written(g, s, n):
+                    if g.pool.holders(page) > 1:
+                        shared[page] = shared.get(page, 0) + 1
+            need += sum(min(w, g.pool.holders(page) - 1) for page, w in shared.items())
             if need > g.pool.free_pages:
                 raise CacheFullError(
                     f"the cache is full: {need} more pages of {PAGE_TOKENS} tokens wanted, {g.pool.free_pages} of {g.pool.n_pages} free")
@@ -223,8 +233,114 @@ class SequenceCache:
                     new = g.pool.take(more)
                     g.pages[s].extend(new)
                     g.table_host[s, have:have + more] = new
-                    lo, hi = g.dirty.get(s, (have, have))
-                    g.dirty[s] = (min(lo, have), max(hi, have + more))
+                    self._mark(g, s, have, have + more)
+            copies: List[Tuple[int, int, int]] = []
+            for s, n in wanted:
+                first = self.lengths[s] // PAGE_TOKENS
+                for i, page in enumerate(self._written(g, s, n), start=first):
+                    if g.pool.holders(page) < 2:
+                        continue
+                    own = g.pool.take(1)[0]
+                    filled = self.lengths[s] - i * PAGE_TOKENS
+                    if filled > 0:
+                        copies.append((page, own, filled))
+                    g.pool.give_back([page])
+                    g.pages[s][i] = own
+                    g.table_host[s, i] = own
+                    self._mark(g, s, i, i + 1)
+            if copies:
+                self._copy_rows(g, copies)
+
+    def _written(self, g: _Group, slot: int, new_len: int) -> List[int]:
+        """The slot's pages, among those it has, that tokens from its length up to `new_len` go to."""
+        if new_len <= self.lengths[slot]:
+            return []
+        return g.pages[slot][self.lengths[slot] // PAGE_TOKENS:pages_for(new_len)]
+
+    @staticmethod
+    def _mark(g: _Group, slot: int, lo: int, hi: int) -> None:
+        was = g.dirty.get(slot, (lo, hi))
+        g.dirty[slot] = (min(was[0], lo), max(was[1], hi))
+
+    def _to_device(self, values) -> torch.Tensor:
+        t = torch.tensor(values, dtype=torch.int32, pin_memory=self.device.type == "cuda")
+        return t.to(self.device, non_blocking=True)
+
+    def _copy_rows(self, g: _Group, copies: Sequence[Tuple[int, int, int]]) -> None:
+        """(page, page to copy to, filled rows), keys and values of all the group's entries, on the current stream."""
+        storage = [t for t in (g.k, g.v) if t is not None]
+        if self.device.type != "cuda":
+            for src, dst, rows in copies:
+                for t in storage:
+                    t[:, dst, :, :rows] = t[:, src, :, :rows]
+            return
+        from ..kernels import ops
+        src, dst, rows = self._to_device([list(x) for x in zip(*copies)]).unbind(0)
+        ops.copy_pages(storage, src, dst, rows)
+
+    # ---- several continuations of one sequence ---------------------------------------------------
+    def fork(self, slot: int) -> int:
+        """Another slot that holds what `slot` holds: the same pages, a copy of its fixed-size state."""
+        if not self.slots.live(slot):
+            raise RuntimeError(f"slot {slot} is not open")
+        new = self.open_slot()
+        for g in self._groups:
+            g.pages[new] = list(g.pages[slot])
+            g.first_live[new] = g.first_live[slot]
+            g.pool.share([p for p in g.pages[new] if p != PagePool.TRASH_PAGE])
+            n = len(g.pages[new])
+            g.table_host[new, :n] = g.pages[new]
+            self._mark(g, new, 0, n)
+        for d in (self._state, self._block_state):
+            for t in d.values():
+                t[new].copy_(t[slot])
+        self.lengths[new] = self.lengths[slot]
+        return new
+
+    def reorder(self, slots: Sequence[Sequence[int]], parents: Sequence[Sequence[int]]) -> None:
+        """Every sequence's slots take over from others of them: slot slots[s][j] holds afterwards what slots[s][parents[s][j]]
+        held before.  Pages are shared, fixed-size states move on the device.  Every sequence has equally many slots."""
+        flat = [s for row in slots for s in row]
+        if len(set(flat)) != len(flat):
+            raise ValueError("a slot is named twice")
+        for row, up in zip(slots, parents):
+            if len(row) != len(slots[0]) or len(up) != len(row) or any(not 0 <= p < len(row) for p in up):
+                raise ValueError("every sequence wants equally many slots, and a parent among them for each")
+        if len(slots) != len(parents):
+            raise ValueError(f"{len(slots)} sequences, parents of {len(parents)}")
+        for s in flat:
+            if not self.slots.live(s):
+                raise RuntimeError(f"slot {s} is not open")
+        moves = [(row[j], row[p]) for row, up in zip(slots, parents) for j, p in enumerate(up) if p != j]
+        if not moves:
+            return
+        was = {s: self.lengths[s] for s in flat}
+        for g in self._groups:
+            old = {s: (g.pages[s], g.first_live[s]) for s in flat}
+            for to, src in moves:
+                g.pool.share([p for p in old[src][0] if p != PagePool.TRASH_PAGE])
+            for to, src in moves:
+                pages = list(old[src][0])
+                g.pool.give_back([p for p in old[to][0] if p != PagePool.TRASH_PAGE])
+                g.pages[to], g.first_live[to] = pages, old[src][1]
+                before, n = old[to][0], len(pages)
+                same = next((i for i, (a, b) in enumerate(zip(before, pages)) if a != b), min(len(before), n))
+                g.table_host[to, n:len(before)] = 0
+                g.table_host[to, same:n] = pages[same:]
+                if same < n:
+                    self._mark(g, to, same, n)
+        for to, src in moves:
+            self.lengths[to] = was[src]
+        states = [t for d in (self._state, self._block_state) for t in d.values()]
+        if not states:
+            return
+        if self.device.type != "cuda":
+            to, src = torch.tensor([m[0] for m in moves]), torch.tensor([m[1] for m in moves])
+            for t in states:
+                t[to] = t[src]
+            return
+        from ..kernels import ops
+        ops.reorder_states(states, self._to_device([list(r) for r in slots]), self._to_device([list(r) for r in parents]))
 
     def commit(self, slot: int, new_len: int) -> None:
         """The slot now holds `new_len` tokens.  Window and chunk groups give back pages no later query can see."""

@@ -42,6 +42,8 @@ OPTIONS:
         --ctx <n>         context window in tokens           [2048]
         --prompt-len <n>  prompt length (bench)              [256]
         --batch <n>       sequences per batch                [run: 8, bench: 1]
+        --beams <n>       run: beam search with n beams, the best result of each prompt
+        --draft <n>       run: greedy, with up to n tokens a step drafted from the sequence itself
         --dtype <t>       bfloat16 or float32                [bfloat16]
         --gpu             accepted for compatibility: there is no other backend
 
@@ -64,6 +66,8 @@ class Opts:
     ctx: Optional[int] = None
     prompt_len: int = 256
     batch: Optional[int] = None
+    beams: int = 0
+    draft: int = 0
     dtype: str = "bfloat16"
     gpu: bool = True
 
@@ -109,6 +113,10 @@ def parse_opts(args: List[str]) -> Opts:
             o.prompt_len = int(num(val(a), a))
         elif a == "--batch":
             o.batch = int(num(val(a), a))
+        elif a == "--beams":
+            o.beams = int(num(val(a), a))
+        elif a == "--draft":
+            o.draft = int(num(val(a), a))
         elif a == "--dtype":
             o.dtype = val(a)
         elif a == "--gpu":
@@ -169,19 +177,29 @@ def cmd_run(o: Opts) -> None:
         raise UsageError("run needs -p <token ids>")
     prompts = parse_ids(o.prompt)
     ctx = o.ctx or 2048
-    batch = o.batch or 8
-    llm = _llm(o, max_tokens=min(batch, len(prompts)) * ctx, ctx=ctx)
+    if o.beams and o.draft:
+        raise UsageError("--beams and --draft do not go together")
+    batch = o.batch or (1 if o.beams else 8)
+    # beams share their prompt's pages; each has pages of its own for what it adds
+    llm = _llm(o, max_tokens=min(batch, len(prompts)) * (ctx + o.beams * (o.max_new + 128)), ctx=ctx)
     if _profile_wanted():          # GHOST_INFER_PROFILE, as the reference's switch is called (src/profile.rs:20-29)
         from .kernels import ops
         ops.profile_start()
-    results = llm.generate(prompts, max_new=o.max_new, temperature=o.temp, top_k=o.top_k, top_p=o.top_p,
-                           seed=o.seed, batch_size=batch)
+    if o.beams:
+        results = [r[0] for r in llm.beam_search(prompts, beams=o.beams, max_new=o.max_new, batch_size=batch)]
+    elif o.draft:
+        results = llm.generate_drafted(prompts, max_new=o.max_new, max_nodes=o.draft + 1, batch_size=batch)
+    else:
+        results = llm.generate(prompts, max_new=o.max_new, temperature=o.temp, top_k=o.top_k, top_p=o.top_p,
+                               seed=o.seed, batch_size=batch)
     for r in results:
         print(" ".join(str(t) for t in r.tokens))
-    print_stats(llm.last_stats)
+    st = llm.last_stats
+    if st is not None:
+        print_stats(st)
     if _profile_wanted():
-        st = llm.last_stats
-        print_profile(ops.profile_stop(), st.prompt_tokens + st.gen_tokens)
+        tokens = st.prompt_tokens + st.gen_tokens if st is not None else sum(map(len, prompts)) + sum(len(r.tokens) for r in results)
+        print_profile(ops.profile_stop(), tokens)
 
 
 def cmd_top(model: str, ids_text: str, dtype: str = "bfloat16") -> None:

@@ -1,4 +1,4 @@
 from .model import Model
-from .step import Engine, StepContext, StepEntry
+from .step import Engine, StepContext, StepEntry, TreeEntry, TreeStep
 
-__all__ = ["Model", "Engine", "StepContext", "StepEntry"]
+__all__ = ["Model", "Engine", "StepContext", "StepEntry", "TreeEntry", "TreeStep"]

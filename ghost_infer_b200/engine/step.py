@@ -7,6 +7,10 @@ Here one call takes several sequences at once: each entry names a slot of the ca
 that sequence (a whole prompt, a chunk of one, or one decoded token) and the places among them whose
 logits are wanted.  Positions follow from the slot's length.  Only the tokens given are run, as one flat
 batch `[total tokens]` with per-sequence offsets; nothing is padded, so padding cannot change a result.
+
+A step may also carry a tree of drafted tokens per sequence (`Engine.step_tree`): every node continues its parent, sees what
+is cached and its ancestors, and has its parent's position plus one.  The nodes' keys and values are stored one after the
+other behind the cached ones; `Engine.commit_tree` keeps those of the nodes that the model's own picks lead through.
 """
 from __future__ import annotations
 
@@ -24,6 +28,46 @@ class StepEntry:
     slot: int
     tokens: Sequence[int]
     want: Sequence[int] = ()      # places among `tokens` whose logits are asked for
+
+
+@dataclass
+class TreeEntry:
+    """A slot's drafted tokens: `tokens[0]` is the token that would be fed anyway; node i continues node `parents[i]`, which comes
+    before it (`parents[0]` is -1)."""
+    slot: int
+    tokens: Sequence[int]
+    parents: Sequence[int]
+
+
+@dataclass
+class TreeFacts:
+    """What the parts see of a step's trees, on the device."""
+    masks: torch.Tensor                     # int32 [T, words]: the nodes of its own tree that a token sees, 32 to a word
+    depth_positions: torch.Tensor           # int32 [T]: position of a token along its path
+    parents: torch.Tensor                   # int32 [T]
+
+
+@dataclass
+class TreeStep:
+    """A step over trees that has run: its logits (a row for every node, in the entries' order), and what `commit_tree` needs."""
+    logits: torch.Tensor
+    context: "StepContext"
+    entries: List[TreeEntry]
+    done: bool = False
+
+
+MAX_TREE_NODES = 256
+
+
+def tree_facts(parents: Sequence[int], words: int):
+    """(mask words uint32 [nodes, words], depths) of one tree."""
+    masks, depths = np.zeros((len(parents), words), dtype=np.uint32), np.zeros(len(parents), dtype=np.int32)
+    for i, p in enumerate(parents):
+        if p >= 0:
+            masks[i] = masks[p]
+            depths[i] = depths[p] + 1
+        masks[i, i // 32] |= np.uint32(1 << (i % 32))
+    return masks, depths
 
 
 class StepContext:
@@ -44,6 +88,7 @@ class StepContext:
         self.seq_lens: torch.Tensor = None      # int32 [B] cached length after the step
         self.logit_rows: Optional[torch.Tensor] = None   # int32 [R] flat token indices
         self.empty_f32: torch.Tensor = None
+        self.tree: Optional[TreeFacts] = None   # a step over trees of drafted tokens
         self.shared: dict = {}                  # what parts compute once per step and share (e.g. rotary angles)
         self.next_reader = None                 # the part that reads the stream next after the one running now, where it says what it does
         self.sm_count = 148
@@ -280,6 +325,67 @@ class Engine:
         """A runner of one-token steps for these slots (see engine.decode.DecodeRunner)."""
         from .decode import DecodeRunner
         return DecodeRunner(self, slots, use_graph=use_graph)
+
+    # ---- trees of drafted tokens ------------------------------------------------------------------
+    def takes_trees(self) -> bool:
+        """Whether `step_tree` can run this model: attention over everything cached in every layer, no fixed-size state."""
+        return (bool(self._mixers) and all(getattr(m, "takes_trees", False) for m in self._mixers)
+                and not self.cache.state_bytes_per_sequence() and all(g.request.kind == "full" for g in self.cache.groups))
+
+    def _validate_trees(self, entries: Sequence[TreeEntry]) -> None:
+        if not self.takes_trees():
+            raise ValueError("this model cannot step over trees of drafted tokens: every layer must attend to all cached positions, "
+                             "and nothing else may be kept per sequence")
+        self._validate([StepEntry(e.slot, e.tokens) for e in entries])
+        for e in entries:
+            n = len(e.tokens)
+            if n > MAX_TREE_NODES:
+                raise ValueError(f"slot {e.slot}: a tree of {n} nodes, at most {MAX_TREE_NODES} are supported")
+            if len(e.parents) != n or e.parents[0] != -1 or any(not 0 <= int(p) < i for i, p in enumerate(e.parents[1:], start=1)):
+                raise ValueError(f"slot {e.slot}: a tree's first node has the parent -1, every other one a node before it")
+
+    def step_tree(self, entries: Sequence[TreeEntry]) -> TreeStep:
+        """Runs every slot's tree of drafted tokens after what the slot holds.  The slots' lengths do not change before
+        `commit_tree`; a step that is not committed leaves nothing behind."""
+        self._validate_trees(entries)
+        self.cache.reserve([(e.slot, self.cache.length(e.slot) + len(e.tokens)) for e in entries])
+        self.cache.sync_tables()
+        ctx = self.build_context([StepEntry(e.slot, e.tokens, range(len(e.tokens))) for e in entries])
+        ctx.is_decode = False
+        words = (ctx.max_q_len + 31) // 32
+        facts = [tree_facts(e.parents, words) for e in entries]
+        packed = np.concatenate([np.concatenate([m for m, _ in facts]).view(np.int32).reshape(-1),
+                                 np.concatenate([d + self.cache.length(e.slot) for (_, d), e in zip(facts, entries)]).astype(np.int32),
+                                 np.concatenate([np.asarray(e.parents, dtype=np.int32) for e in entries])])
+        dev = self._staging.upload(packed) if self._staging is not None else torch.from_numpy(packed).to(self.device)
+        self.bytes_h2d += packed.nbytes
+        T = ctx.n_tokens
+        ctx.tree = TreeFacts(dev[:T * words].view(T, words), dev[T * words:T * words + T], dev[T * words + T:])
+        return TreeStep(self.forward(ctx), ctx, list(entries))
+
+    def commit_tree(self, tree: TreeStep, picks: torch.Tensor) -> List[List[int]]:
+        """Takes over what the picks (int32 [nodes] on the device: the token chosen after each node) agree with: from a tree's first
+        node on, the child whose token is the pick, as long as there is one.  The slots then hold the accepted tokens.
+        Returns, for every entry, the accepted nodes' tokens after the first, and behind them the pick after the last one."""
+        from ..kernels import ops
+        if tree.done:
+            raise RuntimeError("this step has been committed already")
+        ctx = tree.context
+        for e, pos0 in zip(tree.entries, ctx.host_pos0):
+            if not self.cache.slots.live(e.slot) or self.cache.length(e.slot) != pos0:
+                raise RuntimeError(f"slot {e.slot} has moved on since this step")
+        tree.done = True
+        out = None
+        for g in self.cache.groups:
+            storage = [t for t in (g.k, g.v) if t is not None]
+            out = ops.tree_commit(picks, ctx.tokens, ctx.tree.parents, ctx.cu_seqlens, ctx.seq_slots, ctx.seq_pos0, ctx.n_seqs, ctx.max_q_len,
+                                  storage, g.table_dev)
+        path, counts, nexts = (t.cpu().tolist() for t in out)
+        accepted = []
+        for e, nodes, n, last in zip(tree.entries, path, counts, nexts):
+            self.cache.commit(e.slot, self.cache.length(e.slot) + n)
+            accepted.append([int(e.tokens[i]) for i in nodes[1:n]] + [last])
+        return accepted
 
     def step(self, entries: Sequence[StepEntry]) -> Optional[torch.Tensor]:
         """Runs the entries' tokens after what their slots hold.  Returns float32 logits

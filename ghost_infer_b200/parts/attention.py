@@ -51,6 +51,12 @@ class GqaAttention(Mixer):
         return CacheRequest("full", self.n_kv, self.head_dim)
 
     @property
+    def takes_trees(self) -> bool:
+        """Whether a step over trees of drafted tokens can run here: every cached position stays visible, and the position
+        encoding tells a token's position from the place it is stored at."""
+        return not self.window and (self.position is None or getattr(self.position, "takes_trees", False))
+
+    @property
     def plans_on_host(self) -> bool:
         return bool(self.position is not None and self.position.plans_on_host)
 
@@ -100,7 +106,12 @@ class GqaAttention(Mixer):
     def _attend(self, qkv, inside, residual, step, memory) -> None:
         with ops.bucket("attention"):
             att = torch.empty((qkv.shape[0], self.q_dim), dtype=self.rt.dtype, device=qkv.device)
-            ops.attention(qkv, memory, step, self.n_heads, self.n_kv, self.head_dim, self.scale, self.window, att,
-                          plan=step.plan_of(self), rope=inside)
+            tree = getattr(step, "tree", None)
+            if tree is not None:
+                ops.attention_tree(qkv, memory.k, memory.v, memory.block_table, step.cu_seqlens, step.seq_slots, step.seq_pos0, tree.masks,
+                                   step.n_seqs, step.max_q_len, step.max_kv_len, self.n_heads, self.n_kv, self.head_dim, self.scale, att)
+            else:
+                ops.attention(qkv, memory, step, self.n_heads, self.n_kv, self.head_dim, self.scale, self.window, att,
+                              plan=step.plan_of(self), rope=inside)
         with ops.bucket("out matmul"):
             linear(att, self.w_o, out=residual, accumulate=True)

@@ -59,6 +59,7 @@ def rotary_inv_freq(rotary_dim: int, theta: float, scaling: Optional[Mapping]) -
 
 @register("position", "rotary")
 class Rotary(PositionEncoding):
+    takes_trees = True          # angles may belong to other positions than those the keys are stored at
     settles_pending = True      # its kernel adds partial sums a deferred product left in place of row values
 
     def __init__(self, params, prefix=""):
@@ -92,7 +93,8 @@ class Rotary(PositionEncoding):
         # serves every layer that rotates the same way
         table = step.shared.get(self.table_key)
         if table is None:
-            table = ops.rope_table(step.positions, self.inv_freq, self.magnitude)
+            tree = getattr(step, "tree", None)
+            table = ops.rope_table(step.positions if tree is None else tree.depth_positions, self.inv_freq, self.magnitude)
             step.shared[self.table_key] = table
         return table
 
