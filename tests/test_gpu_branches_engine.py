@@ -8,7 +8,11 @@ import torch
 
 import ghost_infer_b200 as gi
 import test_gpu_barovik as tb
+import test_gpu_navalorn as tn
+import test_gpu_nuzinex as tx
 import test_gpu_sofopel as ts
+import test_gpu_torutar as tt
+import test_gpu_vavupel as tv
 from branch_cases import plain_beam_select, plain_walk, random_tree
 from ghost_infer_b200.engine.step import StepEntry, TreeEntry
 from gpu_helpers import check_logits, make_engine, oracle, plain_logits, tokens_for
@@ -224,8 +228,9 @@ def log_prob_by_prompt(engine, prompt, tokens):
 def recurrent_engines():
     for name in sorted(tb.CONFIGS):
         yield "barovik " + name, lambda name=name: tb.engine_for(name, "float32", max_tokens=64 * 60)
-    for name in sorted(ts.CONFIGS):
-        yield "sofopel " + name, lambda name=name: ts.engine_for(name, "float32", max_tokens=64 * 60)
+    for what, module in (("navalorn", tn), ("nuzinex", tx), ("sofopel", ts), ("torutar", tt), ("vavupel", tv)):
+        for name in sorted(module.CONFIGS):
+            yield f"{what} {name}", lambda module=module, name=name: module.engine_for(name, "float32", max_tokens=64 * 60)
 
 
 @pytest.mark.parametrize("which,make", list(recurrent_engines()), ids=lambda x: x if isinstance(x, str) else "")
