@@ -12,6 +12,8 @@
 // register tile of R / 16 rows by 4 keys a thread, sums of values R / 16 rows by 4 numbers for every 64 of the head; a row's 16
 // threads are one half of a warp, so its maximum and sum need no barrier.
 // Bound: 32-bit multiply-adds (4 per query number, key and value) with many rows, the cache's bytes with few.
+#include <type_traits>
+
 #include "api.h"
 #include "attention_tree.cuh"
 
@@ -23,7 +25,7 @@ constexpr int THREADS = 256;
 constexpr int TILE = 64;
 
 template <typename T, int R, int DCH>
-__global__ void __launch_bounds__(THREADS)
+__global__ void __launch_bounds__(THREADS, R == 64 && DCH == 4 ? 1 : 2)
 attn_tree_kernel(const Shape sh, T* __restrict__ out, long ldo, const T* q, long ldq, const T* kcache, const T* vcache, int hd, float scale,
                  float4* __restrict__ part_o, float2* __restrict__ part_ml, int* __restrict__ part_prefix, int vec) {
   constexpr int RT = R / 16;                       // rows a thread works on: ty + 16 i
@@ -50,9 +52,33 @@ attn_tree_kernel(const Shape sh, T* __restrict__ out, long ldo, const T* q, long
     const int tok0 = sh.cu_seqlens[u.b], len = u.pos0 + u.n;
     const int rows_here = min(sh.rows_block, u.n * group - u.row0);
     __syncthreads();
-    for (int i = tid; i < R * hp; i += THREADS) {
-      const int r = i / hp, d = i % hp, row = u.row0 + r;
-      Qs[r * ld + d] = r < rows_here && d < hd ? gi::ldf(q + (size_t)(tok0 + row / group) * ldq + (size_t)(u.kvh * group + row % group) * hd + d) : 0.f;
+    // the queries: a row's 16 threads (the half warp that works on it) fetch it, all of a thread's pieces at once
+    {
+      float4 own[RT][DCH];
+#pragma unroll
+      for (int i = 0; i < RT; ++i) {
+        const int r = ty + 16 * i, row = u.row0 + r, node = row / group;
+        const T* from = q + (size_t)(tok0 + node) * ldq + (size_t)(u.kvh * group + row - node * group) * hd;
+#pragma unroll
+        for (int c = 0; c < DCH; ++c) {
+          const int d = c * 64 + tx * 4;
+          own[i][c] = make_float4(0.f, 0.f, 0.f, 0.f);
+          if (r < rows_here) {
+            if (vec && d < hd) own[i][c] = gi::ld4(from + d);
+            else if (!vec) {
+              if (d < hd) own[i][c].x = gi::ldf(from + d);
+              if (d + 1 < hd) own[i][c].y = gi::ldf(from + d + 1);
+              if (d + 2 < hd) own[i][c].z = gi::ldf(from + d + 2);
+              if (d + 3 < hd) own[i][c].w = gi::ldf(from + d + 3);
+            }
+          }
+        }
+      }
+#pragma unroll
+      for (int i = 0; i < RT; ++i)
+#pragma unroll
+        for (int c = 0; c < DCH; ++c)
+          if (c * 64 + tx * 4 < hp) *reinterpret_cast<float4*>(Qs + (ty + 16 * i) * ld + c * 64 + tx * 4) = own[i][c];
     }
     float m[RT], l[RT], acc[RT][DCH * 4];
 #pragma unroll
@@ -65,6 +91,9 @@ attn_tree_kernel(const Shape sh, T* __restrict__ out, long ldo, const T* q, long
       const int kt = t * TILE;
       const int page = page_of(sh, u.slot, t);
       const size_t base = ((size_t)page * sh.n_kv + u.kvh) * TILE * hd;
+      const bool in_tree = kt + TILE > u.pos0;
+      bool spoiled = false;                        // a node's value that is no number, or infinite
+      auto look = [&](int r, float v) { spoiled |= in_tree && kt + r >= u.pos0 && !(fabsf(v) < INFINITY); };
       __syncthreads();
       if (vec) {
         const int h4 = hd / 4;
@@ -83,6 +112,7 @@ attn_tree_kernel(const Shape sh, T* __restrict__ out, long ldo, const T* q, long
             if (r < TILE) {
               *reinterpret_cast<float4*>(Ks + r * ld + 4 * c) = kx[w];
               *reinterpret_cast<float4*>(Vs + r * ld + 4 * c) = vx[w];
+              look(r, vx[w].x), look(r, vx[w].y), look(r, vx[w].z), look(r, vx[w].w);
             }
           }
         }
@@ -92,15 +122,16 @@ attn_tree_kernel(const Shape sh, T* __restrict__ out, long ldo, const T* q, long
           const bool live = kt + r < len && d < hd;
           Ks[r * ld + d] = live ? gi::ldf(kcache + base + (size_t)r * hd + d) : 0.f;
           Vs[r * ld + d] = live ? gi::ldf(vcache + base + (size_t)r * hd + d) : 0.f;
+          look(r, Vs[r * ld + d]);
         }
       }
-      __syncthreads();
+      const bool careful = __syncthreads_or(spoiled);
       float s[RT][4];
 #pragma unroll
       for (int i = 0; i < RT; ++i)
 #pragma unroll
         for (int j = 0; j < 4; ++j) s[i][j] = 0.f;
-#pragma unroll 4
+#pragma unroll 2
       for (int d = 0; d < hp; d += 4) {
         float4 k4[4];
 #pragma unroll
@@ -117,7 +148,6 @@ attn_tree_kernel(const Shape sh, T* __restrict__ out, long ldo, const T* q, long
           }
         }
       }
-      const bool in_tree = kt + TILE > u.pos0;
 #pragma unroll
       for (int i = 0; i < RT; ++i) {
         const int r = ty + 16 * i;
@@ -154,31 +184,35 @@ attn_tree_kernel(const Shape sh, T* __restrict__ out, long ldo, const T* q, long
       }
       __syncwarp();
       // a node's value that is no number must not reach those that do not see the node: a weight of zero takes nothing
-      for (int j = 0; j < TILE; j += 4) {
-        float4 v4[4][DCH];
+      auto add_up = [&](auto look_twice) {
+#pragma unroll 2
+        for (int j = 0; j < TILE; j += 4) {
+          float4 p4[RT];
 #pragma unroll
-        for (int w = 0; w < 4; ++w)
-#pragma unroll
-          for (int c = 0; c < DCH; ++c)
-            if (c * 64 + tx * 4 < hp) v4[w][c] = *reinterpret_cast<const float4*>(Vs + (j + w) * ld + c * 64 + tx * 4);
-#pragma unroll
-        for (int i = 0; i < RT; ++i) {
-          const float4 p4 = *reinterpret_cast<const float4*>(Ps + (ty + 16 * i) * 68 + j);
-          const float p[4] = {p4.x, p4.y, p4.z, p4.w};
+          for (int i = 0; i < RT; ++i) p4[i] = *reinterpret_cast<const float4*>(Ps + (ty + 16 * i) * 68 + j);
 #pragma unroll
           for (int w = 0; w < 4; ++w) {
-            if (in_tree && p[w] == 0.f) continue;
+            float4 v4[DCH];
 #pragma unroll
             for (int c = 0; c < DCH; ++c)
-              if (c * 64 + tx * 4 < hp) {
-                acc[i][c * 4] = fmaf(p[w], v4[w][c].x, acc[i][c * 4]);
-                acc[i][c * 4 + 1] = fmaf(p[w], v4[w][c].y, acc[i][c * 4 + 1]);
-                acc[i][c * 4 + 2] = fmaf(p[w], v4[w][c].z, acc[i][c * 4 + 2]);
-                acc[i][c * 4 + 3] = fmaf(p[w], v4[w][c].w, acc[i][c * 4 + 3]);
+              v4[c] = c * 64 + tx * 4 < hp ? *reinterpret_cast<const float4*>(Vs + (j + w) * ld + c * 64 + tx * 4) : make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+            for (int i = 0; i < RT; ++i) {
+                    const float p = w == 0 ? p4[i].x : w == 1 ? p4[i].y : w == 2 ? p4[i].z : p4[i].w;
+              if (decltype(look_twice)::value && p == 0.f) continue;
+#pragma unroll
+              for (int c = 0; c < DCH; ++c) {
+                acc[i][c * 4] = fmaf(p, v4[c].x, acc[i][c * 4]);
+                acc[i][c * 4 + 1] = fmaf(p, v4[c].y, acc[i][c * 4 + 1]);
+                acc[i][c * 4 + 2] = fmaf(p, v4[c].z, acc[i][c * 4 + 2]);
+                acc[i][c * 4 + 3] = fmaf(p, v4[c].w, acc[i][c * 4 + 3]);
               }
+            }
           }
         }
-      }
+      };
+      if (!careful) add_up(std::false_type());
+      else add_up(std::true_type());
     }
     const bool whole = t_begin == 0 && t_end == u.tiles;
     const size_t slot2 = 2 * (size_t)blockIdx.x + (t_begin == 0 ? 1 : 0);
@@ -368,7 +402,7 @@ int launch_tree(const Shape& sh, const Plan& p, T* out, long ldo, const T* q, lo
     if (e != cudaSuccess) return gi::fail(GI_ERR_CUDA, "tree attention: %s", cudaGetErrorString(e));
     if (dev >= 0) configured[dev] = true;
   }
-  const int vec = hd % 4 == 0 && ((uintptr_t)k % (4 * sizeof(T))) == 0 && ((uintptr_t)v % (4 * sizeof(T))) == 0;
+  const int vec = hd % 4 == 0 && ldq % 4 == 0 && (((uintptr_t)k | (uintptr_t)v | (uintptr_t)q) % (4 * sizeof(T))) == 0;
   return gi::check(gi::launch(kern, dim3(p.ranges), dim3(THREADS), smem, s, sh, out, ldo, q, ldq, k, v, hd, scale, part_o, part_ml, part_prefix, vec), "tree attention");
 }
 

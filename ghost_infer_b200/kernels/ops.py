@@ -881,7 +881,7 @@ def check_status() -> None:
     clears the kernels' status words; synchronises the device."""
     bad = []
     for name, fn in (("prompt product", gemm_tc_status), ("decode product", gemm_stream_status),
-                     ("prompt attention", attn_prefill_t5_status), ("tree attention", attn_tree_status)):
+                     ("prompt attention", attn_prefill_t5_status)):
         code = fn()
         if code:
             bad.append(f"{name} (wait {code})")
@@ -1059,10 +1059,13 @@ def attn_prefill_t5_pairing(mode: int) -> None:
 
 
 def attn_prefill_t5_status() -> int:
+    """0 if every wait inside the tcgen05 attention kernels was met since the last call (the one over trees': 16 and more);
+    synchronises the device."""
     lib = _bind()
     status = ctypes.c_int(0)
     _check(lib, lib.gi_attn_prefill_t5_status(ctypes.byref(status)), 0)
-    return status.value
+    other = attn_tree_status()
+    return status.value or (16 + other if other else 0)
 
 
 def attn_tree_status() -> int:
