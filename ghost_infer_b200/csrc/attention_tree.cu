@@ -28,7 +28,6 @@ template <typename T, int R, int DCH>
 __global__ void __launch_bounds__(THREADS, R == 64 && DCH == 4 ? 1 : 2)
 attn_tree_kernel(const Shape sh, T* __restrict__ out, long ldo, const T* q, long ldq, const T* kcache, const T* vcache, int hd, float scale,
                  float4* __restrict__ part_o, float2* __restrict__ part_ml, int* __restrict__ part_prefix, int vec) {
-  constexpr int RT = R / 16;                       // rows a thread works on: ty + 16 i
   extern __shared__ __align__(16) float smem[];
   const int hp = (hd + 3) / 4 * 4, ld = hp + 4;    // rows padded: 16 rows' four-number reads fall into different banks
   float* Qs = smem;                                // [R][ld]
@@ -52,6 +51,8 @@ attn_tree_kernel(const Shape sh, T* __restrict__ out, long ldo, const T* q, long
     const int tok0 = sh.cu_seqlens[u.b], len = u.pos0 + u.n;
     const int rows_here = min(sh.rows_block, u.n * group - u.row0);
     __syncthreads();
+    auto work = [&](auto rows_per_thread) {
+    constexpr int RT = decltype(rows_per_thread)::value;     // rows a thread works on: ty + 16 i
     // the queries: a row's 16 threads (the half warp that works on it) fetch it, all of a thread's pieces at once
     {
       float4 own[RT][DCH];
@@ -236,6 +237,10 @@ attn_tree_kernel(const Shape sh, T* __restrict__ out, long ldo, const T* q, long
       }
       if (!whole && tx == 0) part_ml[slot2 * sh.rows_block + r] = make_float2(m[i], l[i]);
     }
+    };
+    // (a unit of few rows, as the last row block of a tree or a small tree's, is not worked on as if it were full)
+    if (rows_here <= 16) work(std::integral_constant<int, 1>());
+    else work(std::integral_constant<int, R / 16>());
     at = u.first + t_end;
   }
 }
@@ -374,7 +379,7 @@ Plan plan_of(int n_seqs, int max_nodes, int max_kv_len, int n_heads, int n_kv, b
   const long rows = (long)max_nodes * group;
   p.rows_block = tensor ? 128 / group * group : (rows > 16 ? 64 : 16);
   p.tile = tensor ? 128 : TILE;
-  p.least = tensor ? 1 : 2;
+  p.least = 1;
   const long blocks = (rows + p.rows_block - 1) / p.rows_block, rounds = tensor ? (blocks + 7) / 8 : blocks;
   p.split = (int)((blocks + rounds - 1) / rounds);
   const long units = (long)n_seqs * n_kv * rounds, tiles = (max_kv_len + p.tile - 1) / p.tile;
