@@ -2943,12 +2943,11 @@ def beam_select(logits: torch.Tensor, scores: torch.Tensor, width: int):
         raise KernelError(f"{seqs} sequences of {beams} beams want {seqs * beams} rows of logits, got {rows}")
     if not 1 <= width <= MAX_BEAM_WIDTH or width > beams * vocab:
         raise KernelError(f"a width of {width}: 1 to {MAX_BEAM_WIDTH} and at most beams x vocabulary are supported")
-    device = logits.device
-    out = torch.empty((seqs, width), dtype=torch.float32, device=device)
-    parents = torch.empty((seqs, width), dtype=torch.int32, device=device)
+    out = scores.new_empty((seqs, width))
+    parents = torch.empty_like(out, dtype=torch.int32)
     tokens = torch.empty_like(parents)
     nbytes = lib.gi_beam_select_scratch(rows, vocab, width)
-    scratch = torch.empty((nbytes,), dtype=torch.uint8, device=device)
+    scratch = scores.new_empty((nbytes // 4,))
     _check(lib, lib.gi_beam_select(out.data_ptr(), parents.data_ptr(), tokens.data_ptr(), logits.data_ptr(), dt, ld, scores.data_ptr(), seqs, beams, vocab,
                                    width, scratch.data_ptr(), nbytes, stream), 2 if seqs else 0)
     return out, parents, tokens
@@ -3037,7 +3036,7 @@ def attention_tree(q: torch.Tensor, kcache: torch.Tensor, vcache: torch.Tensor, 
         raise KernelError(f"masks of {masks.shape[0]} tokens for {rows}")
     cu, ss, sp = _i32_of(cu_seqlens, n_seqs + 1, "cu_seqlens"), _i32_of(seq_slots, n_seqs, "slots"), _i32_of(seq_pos0, n_seqs, "start positions")
     nbytes = lib.gi_attn_tree_scratch(n_seqs, max_nodes, max_kv_len, n_heads, n_kv, head_dim, dt)
-    scratch = torch.empty((nbytes,), dtype=torch.uint8, device=q.device)
+    scratch = masks.new_empty((nbytes // 4,))
     _check(lib, lib.gi_attn_tree(out.data_ptr(), ldo, q.data_ptr(), ldq, rows, dt, kcache.data_ptr(), vcache.data_ptr(), kcache.shape[0],
                                  _i32_rows(block_table, "block table"), block_table.shape[1], cu, ss, sp, mp, masks.shape[1], n_seqs, max_nodes,
                                  max_kv_len, n_heads, n_kv, head_dim, scale, scratch.data_ptr(), nbytes, stream), 2 if n_seqs else 0)
@@ -3060,9 +3059,8 @@ def tree_commit(picks: torch.Tensor, tokens: torch.Tensor, parents: torch.Tensor
     cu, ss, sp = _i32_of(cu_seqlens, n_seqs + 1, "cu_seqlens"), _i32_of(seq_slots, n_seqs, "slots"), _i32_of(seq_pos0, n_seqs, "start positions")
     if not 1 <= max_nodes <= MAX_TREE_NODES:
         raise KernelError(f"trees of up to {max_nodes} nodes: 1 to {MAX_TREE_NODES} are supported")
-    device = picks.device
-    path = torch.empty((n_seqs, max_nodes), dtype=torch.int32, device=device)
-    counts = torch.empty((n_seqs,), dtype=torch.int32, device=device)
+    path = picks.new_empty((n_seqs, max_nodes))
+    counts = picks.new_empty((n_seqs,))
     nexts = torch.empty_like(counts)
     _check(lib, lib.gi_tree_commit(path.data_ptr(), counts.data_ptr(), nexts.data_ptr(), pk, tk, pr, cu, ss, sp, n_seqs, max_nodes,
                                    _page_tensors(pages, "tree commit"), len(pages), _i32_rows(block_table, "block table"), block_table.shape[1], stream),
