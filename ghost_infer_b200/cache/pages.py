@@ -37,6 +37,7 @@ class PagePool:
         self.n_pages = n_pages            # usable pages, numbered 1..n_pages
         self._free: List[int] = list(range(n_pages, 0, -1))
         self._holders = [0] * (n_pages + 1)
+        self.shared = 0                   # holders beyond the first, over all pages
 
     @property
     def free_pages(self) -> int:
@@ -59,6 +60,7 @@ class PagePool:
             if p <= 0 or p > self.n_pages or not self._holders[p]:
                 raise RuntimeError(f"page {p} is shared but not held")
             self._holders[p] += 1
+            self.shared += 1
 
     def give_back(self, pages: Sequence[int]) -> None:
         for p in pages:
@@ -67,6 +69,8 @@ class PagePool:
             self._holders[p] -= 1
             if not self._holders[p]:
                 self._free.append(p)
+            else:
+                self.shared -= 1
 
 
 class SlotAllocator:

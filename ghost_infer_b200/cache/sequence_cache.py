@@ -217,7 +217,7 @@ class SequenceCache:
         for g in self._groups:
             need = sum(max(0, pages_for(n) - len(g.pages[s])) for s, n in wanted)
             shared: Dict[int, int] = {}                     # page held by others too -> how many of `wanted` want it for themselves
-            for s, n in wanted:
+            for s, n in wanted if g.pool.shared else ():
                 for page in self._written(g, s, n):
                     if g.pool.holders(page) > 1:
                         shared[page] = shared.get(page, 0) + 1
@@ -235,7 +235,7 @@ class SequenceCache:
                     g.table_host[s, have:have + more] = new
                     self._mark(g, s, have, have + more)
             copies: List[Tuple[int, int, int]] = []
-            for s, n in wanted:
+            for s, n in wanted if g.pool.shared else ():
                 first = self.lengths[s] // PAGE_TOKENS
                 for i, page in enumerate(self._written(g, s, n), start=first):
                     if g.pool.holders(page) < 2:

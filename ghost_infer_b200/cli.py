@@ -177,6 +177,8 @@ def cmd_run(o: Opts) -> None:
         raise UsageError("run needs -p <token ids>")
     prompts = parse_ids(o.prompt)
     ctx = o.ctx or 2048
+    if o.beams < 0 or o.draft < 0:
+        raise UsageError("--beams and --draft want a positive number")
     if o.beams and o.draft:
         raise UsageError("--beams and --draft do not go together")
     batch = o.batch or (1 if o.beams else 8)

@@ -433,7 +433,7 @@ extern "C" int gi_attn_tree(void* out, long ldo, const void* q, long ldq, long q
                             const int* block_table, int max_pages, const int* cu_seqlens, const int* seq_slots, const int* seq_pos0, const int* masks,
                             int words, int n_seqs, int max_nodes, int max_kv_len, int n_heads, int n_kv, int hd, float scale, void* scratch,
                             long scratch_bytes, void* stream) {
-  if (n_seqs <= 0) return GI_OK;
+  if (n_seqs <= 0 || q_rows <= 0) return GI_OK;
   if (n_kv < 1 || n_heads < 1 || n_heads % n_kv != 0) return gi::fail(GI_ERR_ARG, "tree attention: %d heads do not divide into %d kv heads", n_heads, n_kv);
   if (hd < 1 || hd > 256) return gi::fail(GI_ERR_UNSUPPORTED, "tree attention: head size %d, 1 to 256 are supported", hd);
   if (max_nodes < 1 || max_nodes > MAX_NODES) return gi::fail(GI_ERR_ARG, "tree attention: trees of up to %d nodes, 1 to %d are supported", max_nodes, MAX_NODES);

@@ -2,7 +2,8 @@
 //
 // Beam j of a sequence carries the score s_j (a sum of log probabilities); token v after it is worth
 //     c(j, v) = s_j + x_jv - ln sum_u exp(x_ju)
-// and the `width` largest of a sequence's beams x vocabulary are wanted in order, ties to the lowest j * V + v.  One pass over
+// and the `width` largest of a sequence's beams x vocabulary are wanted in order; of equal ones the lowest beam's first, within a
+// beam the larger logit (64 bits may not tell two sums apart whose logits differ), then the lowest token.  One pass over
 // the logits does both halves: the sum of exponentials, and the `width` largest logits (within a row the logits' order is the
 // candidates').  A second kernel joins a sequence's rows: their log sums, then the `width` largest candidates of all lists,
 // compared in 64 bits, so that the order between two beams does not hang on the rounding of a sum.
@@ -129,7 +130,7 @@ __device__ __forceinline__ void cut_down(Lists& s, int width) {
   __syncthreads();
 }
 
-// part_stat [row][parts]: (reference in powers of two, sum of 2^(x log2 e - reference)); part_key [row][parts][width]: logits in descending order as
+// part_stat [row][parts]: (reference, sum of exp(x - reference)); part_key [row][parts][width]: logits in descending order as
 // (order of the value, ~token), 0 where there are no more.
 template <typename T>
 __global__ void __launch_bounds__(THREADS, 3)
@@ -190,6 +191,7 @@ beam_rows_kernel(const T* logits, long ld, int vocab, int rows, Cut cut, int wid
   Place part = here;                                 // the part's first tile
   int summed = here.left;                            // the sums hold every tile with more than that many left
   int next_cut = 1;                                  // tiles of the part after which its list is cut down
+  bool wild = false;                                 // a maximum of this thread's was too large to be scaled
   float ref = 0.f, sum = 0.f;                        // of this thread's numbers: sum of 2^(x log2 e - ref)
   bool keep_bar = false, careful = false;            // a part that is gone through again, and what for
   while (here.left > 0) {
@@ -229,7 +231,7 @@ beam_rows_kernel(const T* logits, long ld, int vocab, int rows, Cut cut, int wid
         if (!keep_bar) s.bar = (u64)bar << 32;
       }
       next_cut = 1;
-      if (summed == here.left) ref = 0.f, sum = 0.f;
+      if (summed == here.left) ref = 0.f, sum = 0.f, wild = false;
       __syncthreads();
     }
     if (summed == here.left) {
@@ -237,6 +239,7 @@ beam_rows_kernel(const T* logits, long ld, int vocab, int rows, Cut cut, int wid
       if (mine > -INFINITY) {
         // (scaled, unless it is too large for that: those parts are gone through carefully, with the reference itself)
         const float top = careful ? mine : mine * LOG2E;
+        wild |= !(fabsf(top) < INFINITY);
         if (top > ref || sum == 0.f) {
           sum = sum == 0.f ? 0.f : sum * ex2(careful ? (ref - top) * LOG2E : ref - top);
           ref = top;
@@ -293,7 +296,7 @@ beam_rows_kernel(const T* logits, long ld, int vocab, int rows, Cut cut, int wid
     const float own_ref = sum != 0.f ? ref : -INFINITY;
     float top_ref = gi::warp_max(own_ref);
     if (lane == 0) s_ref[warp] = top_ref;
-    const bool none = __syncthreads_or(!(fabsf(sum) < INFINITY) || (sum != 0.f && !(fabsf(ref) < INFINITY)));
+    const bool none = __syncthreads_or(wild || !(fabsf(sum) < INFINITY));
     if (none && !careful) {
       careful = keep_bar = true;                       // (the bar that the list ended with is reached by `width` logits)
       summed = part.left;
@@ -315,7 +318,7 @@ beam_rows_kernel(const T* logits, long ld, int vocab, int rows, Cut cut, int wid
     if (tid == 0) {
       double t = 0.0;
       for (int w = 0; w < WARPS; ++w) t += s_sum[w];
-      part_stat[out] = make_double2(careful ? (double)top_ref * 1.4426950408889634 : (double)top_ref, t);
+      part_stat[out] = make_double2(careful ? (double)top_ref : (double)top_ref * 0.69314718055994530942, t);
     }
     keep_bar = careful = false;
     part = here;
@@ -323,11 +326,14 @@ beam_rows_kernel(const T* logits, long ld, int vocab, int rows, Cut cut, int wid
   gi::cp_async_wait<0>();
 }
 
-// A candidate of the join: worth more, or as much and earlier among beams x vocabulary.
+// A candidate of the join: its worth, beam and entry (logit and token).
 struct Candidate {
   double c;
-  long at;
-  __device__ __forceinline__ bool before(const Candidate& o) const { return c > o.c || (c == o.c && at < o.at); }
+  u64 key;
+  int beam;
+  __device__ __forceinline__ bool before(const Candidate& o) const {
+    return c > o.c || (c == o.c && (beam < o.beam || (beam == o.beam && key > o.key)));
+  }
 };
 
 // Order of doubles as order of unsigned numbers.
@@ -340,13 +346,15 @@ __device__ __forceinline__ u64 order_key(double v) {
 // side: for a bar that `width` of them reach (as in the rows' first tiles, on the upper halves of the candidates' keys), and for
 // those that reach it, which are put in order by counting.
 __global__ void __launch_bounds__(THREADS)
-beam_join_kernel(const float* scores, const double2* part_stat, const u64* part_key, int beams, Cut cut, int width, int vocab,
+beam_join_kernel(const float* scores, const double2* part_stat, const u64* part_key, int beams, Cut cut, int width,
                  float* __restrict__ out_scores, int* __restrict__ out_parents, int* __restrict__ out_tokens) {
   constexpr int AHEAD = 4;
   __shared__ double s_base[MAX_BEAMS];
   __shared__ int s_parts[MAX_BEAMS];              // parts that a row has
   __shared__ Lists s;
-  __shared__ Candidate s_passed[CAP];
+  __shared__ double s_c[CAP];                     // the candidates that pass: worth, and what orders equal ones
+  __shared__ u64 s_key[CAP];
+  __shared__ int s_beam[CAP];
   __shared__ Candidate s_best[WARPS];
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int seq = blockIdx.x, parts = cut.parts, entries = beams * parts * width;
@@ -383,16 +391,16 @@ beam_join_kernel(const float* scores, const double2* part_stat, const u64* part_
     for (int p = lane; p < s_parts[j]; p += 32) {
       const double2 v = st[p];
       const double both = fmax(top, v.x);
-      if (both > -INFINITY) sum = (top > -INFINITY ? sum * exp2(top - both) : 0.0) + (v.x > -INFINITY ? v.y * exp2(v.x - both) : v.y);
+      if (both > -INFINITY) sum = (top > -INFINITY ? sum * exp(top - both) : 0.0) + (v.x > -INFINITY ? v.y * exp(v.x - both) : v.y);
       top = both;
     }
     double both = top;
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) both = fmax(both, __shfl_xor_sync(0xffffffffu, both, o));
-    sum = top > -INFINITY ? sum * exp2(top - both) : sum;
+    sum = top > -INFINITY ? sum * exp(top - both) : sum;
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-    const double base = score - (both * 0.69314718055994530942 + log(sum));
+    const double base = score - (both + log(sum));
     if (lane == 0) s_base[j] = isfinite(base) ? base : -INFINITY;      // nothing but -inf, or a logit that is +inf: the beam offers nothing
   }
   __syncthreads();
@@ -400,7 +408,7 @@ beam_join_kernel(const float* scores, const double2* part_stat, const u64* part_
     const double base = s_base[j];
     Candidate own;
     own.c = key == 0 || !(base > -INFINITY) ? -INFINITY : base + (double)key_value((unsigned)(key >> 32));
-    own.at = (long)j * vocab + (long)(~(unsigned)(key & 0xffffffffu));
+    own.key = key, own.beam = j;
     return own;
   };
   auto entry = [&](int q, int e) {                  // the q-th of this thread's entries
@@ -423,7 +431,7 @@ beam_join_kernel(const float* scores, const double2* part_stat, const u64* part_
   auto pass = [&](const Candidate& own) {
     if (!(own.c > -INFINITY) || (unsigned)(order_key(own.c) >> 32) < bar) return;
     const int at = atomicAdd(&s.passed_count, 1);
-    if (at < CAP) s_passed[at] = own;
+    if (at < CAP) s_c[at] = own.c, s_key[at] = own.key, s_beam[at] = own.beam;
   };
 #pragma unroll
   for (int q = 0; q < AHEAD; ++q) pass(entry(q, 0));
@@ -433,28 +441,32 @@ beam_join_kernel(const float* scores, const double2* part_stat, const u64* part_
   auto store = [&](int place, const Candidate& own) {
     const size_t o = (size_t)seq * width + place;
     const bool none = !(own.c > -INFINITY);
-    const int parent = none ? -1 : (int)(own.at / vocab);
     out_scores[o] = (float)own.c;
-    out_parents[o] = parent;
-    out_tokens[o] = none ? -1 : (int)(own.at - (long)parent * vocab);
+    out_parents[o] = none ? -1 : own.beam;
+    out_tokens[o] = none ? -1 : (int)(~(unsigned)(own.key & 0xffffffffu));
   };
   Candidate none;
-  none.c = -INFINITY, none.at = 0;
+  none.c = -INFINITY, none.key = 0, none.beam = 0x7fffffff;
   if (count <= CAP) {
     for (int i = tid; i < count; i += THREADS) {
-      const Candidate own = s_passed[i];
+      Candidate own;
+      own.c = s_c[i], own.key = s_key[i], own.beam = s_beam[i];
       int place = 0;
-      for (int o = 0; o < count; ++o) place += s_passed[o].before(own) ? 1 : 0;
+#pragma unroll 4
+      for (int o = 0; o < count; ++o) {
+        const double c = s_c[o];
+        if (c > own.c) ++place;
+        else if (c == own.c && o != i) place += s_beam[o] < own.beam || (s_beam[o] == own.beam && s_key[o] > own.key) ? 1 : 0;
+      }
       if (place < width) store(place, own);
     }
     for (int i = count + tid; i < width; i += THREADS) store(i, none);
     return;
   }
   Candidate last;                                   // (many equal candidates: `width` rounds of a block maximum)
-  last.c = INFINITY, last.at = -1;
+  last.c = INFINITY, last.key = ~(u64)0, last.beam = -1;
   for (int r = 0; r < width; ++r) {
     Candidate best = none;
-    best.at = 0x7fffffffffffffffL;
     for (int e = tid; e < entries; e += THREADS) {
       const Candidate own = entry(AHEAD, e);
       if (own.c > -INFINITY && last.before(own) && own.before(best)) best = own;
@@ -463,7 +475,8 @@ beam_join_kernel(const float* scores, const double2* part_stat, const u64* part_
     for (int o = 16; o > 0; o >>= 1) {
       Candidate other;
       other.c = __shfl_xor_sync(0xffffffffu, best.c, o);
-      other.at = __shfl_xor_sync(0xffffffffu, best.at, o);
+      other.key = __shfl_xor_sync(0xffffffffu, best.key, o);
+      other.beam = __shfl_xor_sync(0xffffffffu, best.beam, o);
       if (other.before(best)) best = other;
     }
     if (lane == 0) s_best[warp] = best;
@@ -535,6 +548,6 @@ extern "C" int gi_beam_select(float* out_scores, int* out_parents, int* out_toke
   int rc = GI_OK;
   GI_DISPATCH_DTYPE(dtype, T, rc = launch_rows((const T*)logits, ld, vocab, rows, p, width, stat, key, s));
   if (rc != GI_OK) return rc;
-  return gi::check(gi::launch(beam_join_kernel, dim3(seqs), dim3(THREADS), 0, s, scores, stat, key, beams, p.cut, width, vocab, out_scores,
+  return gi::check(gi::launch(beam_join_kernel, dim3(seqs), dim3(THREADS), 0, s, scores, stat, key, beams, p.cut, width, out_scores,
                               out_parents, out_tokens), "beam selection (join)");
 }

@@ -364,7 +364,8 @@ class Engine:
         return TreeStep(self.forward(ctx), ctx, list(entries))
 
     def commit_tree(self, tree: TreeStep, picks: torch.Tensor) -> List[List[int]]:
-        """Takes over what the picks (int32 [nodes] on the device: the token chosen after each node) agree with: from a tree's first
+        """Takes over what the picks (int32 [nodes] on the device, in the order of the logits' rows: the token chosen after each node)
+        agree with: from a tree's first
         node on, the child whose token is the pick, as long as there is one.  The slots then hold the accepted tokens.
         Returns, for every entry, the accepted nodes' tokens after the first, and behind them the pick after the last one."""
         from ..kernels import ops
@@ -374,12 +375,12 @@ class Engine:
         for e, pos0 in zip(tree.entries, ctx.host_pos0):
             if not self.cache.slots.live(e.slot) or self.cache.length(e.slot) != pos0:
                 raise RuntimeError(f"slot {e.slot} has moved on since this step")
-        tree.done = True
         out = None
         for g in self.cache.groups:
             storage = [t for t in (g.k, g.v) if t is not None]
             out = ops.tree_commit(picks, ctx.tokens, ctx.tree.parents, ctx.cu_seqlens, ctx.seq_slots, ctx.seq_pos0, ctx.n_seqs, ctx.max_q_len,
                                   storage, g.table_dev)
+        tree.done = True
         path, counts, nexts = (t.cpu().tolist() for t in out)
         accepted = []
         for e, nodes, n, last in zip(tree.entries, path, counts, nexts):

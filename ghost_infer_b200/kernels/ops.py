@@ -2927,7 +2927,7 @@ def _i32_rows(t: torch.Tensor, what: str) -> int:
 
 def beam_select(logits: torch.Tensor, scores: torch.Tensor, width: int):
     """Beam search's choice: of every sequence's beams x vocabulary the `width` largest of score + log softmax(logits), in
-    descending order, compared in 64 bits, ties to the lowest beam and then the lowest token.  logits [sequences * beams, vocab]
+    descending order, compared in 64 bits; of equal ones the lowest beam's first, then the larger logit, then the lowest token.  logits [sequences * beams, vocab]
     (float32 or bfloat16, contiguous rows), scores float32 [sequences, beams].  Returns scores float32, parents int32 (the
     beam that goes on) and tokens int32, each [sequences, width]; where no candidate is left: -inf, -1, -1.  A logit that is
     no number counts as -inf; a beam whose logits are all -inf or hold a +inf, or whose score is not finite, offers nothing."""
@@ -2939,6 +2939,8 @@ def beam_select(logits: torch.Tensor, scores: torch.Tensor, width: int):
         raise KernelError("the beams' scores must be contiguous float32 [sequences, beams]")
     seqs, beams = scores.shape
     rows, vocab = logits.shape
+    if rows == 1:
+        ld = max(ld, vocab)           # (one row's distance to the next means nothing)
     if rows != seqs * beams:
         raise KernelError(f"{seqs} sequences of {beams} beams want {seqs * beams} rows of logits, got {rows}")
     if not 1 <= width <= MAX_BEAM_WIDTH or width > beams * vocab:

@@ -22,7 +22,11 @@ def plain_beam_select(logits, scores, width):
                 continue
             value[j] = (scores[s, j] - (top + math.log(np.exp(x - top).sum()))) + x
         flat = value.reshape(-1)
-        order = np.argsort(-flat, kind="stable")[:width]
+        # descending; of equal ones the lowest beam's first, then the larger logit (whose sum 64 bits may not tell apart), then the
+        # lowest token; -0 and 0 are equal
+        x = np.nan_to_num(logits[s * beams:(s + 1) * beams], nan=-np.inf, posinf=np.inf, neginf=-np.inf).reshape(-1) + 0.0
+        place = np.arange(flat.size)
+        order = np.lexsort((place % vocab, -x, place // vocab, -flat))[:width]
         none = ~np.isfinite(flat[order])
         out.append((flat[order], np.where(none, -1, order // vocab), np.where(none, -1, order % vocab)))
     return tuple(np.stack([row[i] for row in out]) for i in range(3))

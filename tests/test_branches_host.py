@@ -20,12 +20,12 @@ def test_a_page_goes_back_with_its_last_holder():
     a, b = pool.take(2)
     pool.share([a])
     pool.share([a, b])
-    assert pool.holders(a) == 3 and pool.holders(b) == 2 and pool.free_pages == 2
+    assert pool.holders(a) == 3 and pool.holders(b) == 2 and pool.free_pages == 2 and pool.shared == 3
     pool.give_back([a, b])
     pool.give_back([a])
     assert pool.free_pages == 2 and pool.holders(a) == 1
     pool.give_back([b, a])
-    assert pool.free_pages == 4
+    assert pool.free_pages == 4 and pool.shared == 0
     for bad in ([a], [0], [5]):
         with pytest.raises(RuntimeError):
             pool.share(bad)
@@ -270,6 +270,7 @@ def test_refusals_without_a_gpu():
 def test_command_line_options():
     o = cli.parse_opts(["m", "--beams", "4", "--draft", "16"])
     assert (o.beams, o.draft) == (4, 16)
-    with pytest.raises(cli.UsageError):
-        cli.cmd_run(cli.parse_opts(["m", "-p", "1", "--beams", "4", "--draft", "16"]))
+    for args in (["--beams", "4", "--draft", "16"], ["--beams", "-1"], ["--draft", "-2"]):
+        with pytest.raises(cli.UsageError):
+            cli.cmd_run(cli.parse_opts(["m", "-p", "1"] + args))
     assert plain_walk([], [], []) == ([], -1)

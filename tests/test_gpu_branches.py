@@ -383,6 +383,48 @@ def test_tree_attention_rows_strides_and_padding(dtype, dim):
     c.check(c.run(max_kv_len=100000))
 
 
+@pytest.mark.parametrize("dtype,dim,shift", [(BF16, 128, 1), (BF16, 64, 4), (F32, 64, 1), (BF16, 128, 8)])
+def test_tree_attention_rows_on_any_boundary(dtype, dim, shift):
+    """Queries and output that start on no 16-byte boundary, rows whose distance is no multiple of one."""
+    c = TreeCase([9, 40], [130, 77], 4, 2, dim, dtype, seed=9)
+    want = c.run()
+    q = torch.zeros((49, 4 * dim + shift), dtype=dtype, device=DEV)
+    q[:, shift:] = c.q
+    wide = torch.zeros((49, 4 * dim + 2 * shift), dtype=dtype, device=DEV)
+    c.check(c.run(q=q[:, shift:]))
+    c.check(c.run(out=wide[:, shift:shift + 4 * dim]))
+    c.check(c.run(q=q[:, shift:], out=wide[:, shift:shift + 4 * dim]))
+    assert (wide[:, :shift] == 0).all() and (wide[:, shift + 4 * dim:] == 0).all()
+    c.check(want)
+
+
+def test_calls_with_nothing_to_do():
+    none = i32([])
+    out = torch.zeros((0, 64), dtype=BF16, device=DEV)
+    pages = torch.zeros((2, 1, 64, 64), dtype=BF16, device=DEV)
+    masks = torch.zeros((0, 1), dtype=torch.int32, device=DEV)
+    for n in (0, 2):
+        ops.attention_tree(out, pages, pages, i32([[1]]), i32([0] * (n + 1)), i32([0] * n), i32([5] * n), masks, n, 1, 64, 1, 1, 64, 1.0, out)
+        path, counts, nexts = ops.tree_commit(none, none, none, i32([0] * (n + 1)), i32([0] * n), i32([5] * n), n, 4, [pages[None]], i32([[1]]))
+        assert path.tolist() == [[-1] * 4] * n and counts.tolist() == [0] * n and nexts.tolist() == [-1] * n
+    got = ops.beam_select(torch.zeros((0, 9), device=DEV), torch.zeros((0, 3), device=DEV), 4)
+    assert all(tuple(t.shape) == (0, 4) for t in got)
+    ops.reorder_states([torch.zeros((3, 4), device=DEV)], i32([]).view(0, 2), i32([]).view(0, 2))
+    one = torch.randn(50, device=DEV).as_strided((1, 50), (1, 1))
+    check_beams(one, torch.zeros(1, 1, device=DEV), 3)
+
+
+def test_beam_select_logits_of_any_size():
+    """Logits too large to be scaled, rows that hold both ends, a row of one value, numbers around zero."""
+    g = torch.Generator().manual_seed(0)
+    big = (torch.rand(4, 9000, generator=g) * 2 - 1) * 3.3e38
+    big[2] = big[2].abs()
+    big[3, 1:] = -3.3e38
+    check_beams(big.to(DEV), torch.zeros(2, 2, device=DEV), 8)
+    tiny = (torch.rand(2, 9000, generator=g) - 0.5) * 1e-37
+    check_beams(tiny.to(DEV), torch.zeros(1, 2, device=DEV), 64)
+
+
 @pytest.mark.parametrize("dtype,dim", [(F32, 64), (BF16, 128)])
 def test_tree_attention_one_long_context_over_all_blocks(dtype, dim):
     """One kv head and one sequence: its tiles lie on every block, and many parts are joined."""
