@@ -17,8 +17,9 @@
 // lies behind the last node is overwritten with zeros in shared memory, and so is a node's value row that holds an infinity or no
 // number; the rows that do see such a node get no number for an answer (in all of the head's numbers, not in the spoiled ones alone).
 //
-// Bound: the cache's bytes (64 KB a tile at head size 128 take an SM's share of the memory about 2,850 cycles; products take 1,024,
-// exponentials 1,170).  Every wait has an iteration limit.
+// Bound: the cache's bytes with up to 128 rows (64 KB a tile at head size 128 take an SM's share of the memory about 2,850 cycles;
+// products take 1,200, the row threads 2,400), the row threads with more.  B200, 32 heads of 128 over 8, 8 sequences behind 8,192
+// positions: 1 node 56 us, 32 nodes 60 us (4.5 TB/s), 64 nodes 86 us (0.8 PFLOP/s).  Every wait has an iteration limit.
 #include <cuda.h>
 
 #include "api.h"
@@ -185,11 +186,13 @@ attn_tree_t5_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
     const bool keys = warp == 8;
     const CUtensorMap* map = keys ? &map_k : &map_v;
     const uint32_t full = keys ? k_full : v_full, empty = keys ? k_empty : v_empty, stages = smem_u32(smem + (keys ? L::K_AT : L::V_AT));
+    int asked = 0, copied = 0;                      // units' queries, tiles
     for (; ok && next_unit(at, u, t_begin, t_end); ++f) {
       const int pages = (u.pos0 + u.n + PAGE_TOKENS - 1) / PAGE_TOKENS;
       if (keys && lane == 0) {
         if (f > 0) ok = mbar_wait(q_empty, (uint32_t)((f - 1) & 1), 1, &g_tree_status);
         if (ok) {
+          ++asked;
           // rows of a box: a node's heads one below the other (a row past the sequence's nodes belongs to nobody and is not looked at)
           const int node = sh.cu_seqlens[u.b] + u.row0 / group;
           mbar_expect_tx(q_full, HALVES * q_box * 128);
@@ -209,18 +212,21 @@ attn_tree_t5_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
           if (lane == 0) {
             if (j >= STAGES) ok = mbar_wait(empty + 8 * s, (uint32_t)((j / STAGES - 1) & 1), 1, &g_tree_status);
             if (ok) {
+              ++copied;
               mbar_expect_tx(full + 8 * s, L::BYTES_TILE);
 #pragma unroll
               for (int x = 0; x < 2 * HALVES; ++x)
                 tma_load_2d(stages + s * L::BYTES_TILE + (x >> 1) * HALF + (x & 1) * (HALF / 2), map, (x >> 1) * 64, row[x & 1], full + 8 * s);
-            } else {
-              // giving up: the copies under way must have landed before the block's shared memory goes to another one
-              for (int t = max(0, j - STAGES); t < j; ++t) mbar_wait(full + 8 * (t % STAGES), (uint32_t)((t / STAGES) & 1), 1, &g_tree_status);
             }
           }
           ok = __shfl_sync(0xffffffffu, ok ? 1 : 0, 0) != 0;
         }
       }
+    }
+    // whoever gave up in this block: copies under way land before its shared memory goes to another one
+    if (lane == 0) {
+      if (asked > 0) mbar_wait(q_full, (uint32_t)((asked - 1) & 1), 1, &g_tree_status);
+      for (int t = max(0, copied - STAGES); t < copied; ++t) mbar_wait(full + 8 * (t % STAGES), (uint32_t)((t / STAGES) & 1), 1, &g_tree_status);
     }
   } else if (warp == 9) {
     // ---- score products
