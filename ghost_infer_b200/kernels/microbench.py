@@ -7,7 +7,8 @@ Kernels: gemm_stream, gemm_skinny (decode products), gemm_tc (prefill product), 
 attn_prefill_t5 (tcgen05), attn_latent_decode, attn_latent_prefill (attention over one shared latent row per position:
 --heads, --rank, --rot-dim),
 linear_state, mamba2_scan (the token-by-token recurrences: --batch, --context, --heads, --kv-heads, --head-dim, --v-dim,
---delta), rmsnorm, rope, sample.  Operands rotate through enough different buffers to exceed the L2 cache, so a bytes
+--delta), attn_tree (trees of --nodes drafted tokens behind --context positions), beam_select (--batch sequences of --beams beams over
+--n tokens, --width candidates), rmsnorm, rope, sample.  Operands rotate through enough different buffers to exceed the L2 cache, so a bytes
 figure is a DRAM figure.  The same command under `ncu --clock-control none -k regex:<kernel> -c 3` profiles exactly these launches.
 The reference times whole runs only (`bench`, src/main.rs:1241-1285) and, per operation, wall-clock buckets
 (src/profile.rs:7-46); per-kernel device timing is what a roofline needs.
@@ -72,6 +73,9 @@ def main() -> int:
     ap.add_argument("--stages", type=int, default=0, help="attn_decode: depth of each warp's ring of tiles (2 to 4)")
     ap.add_argument("--keys-on-rows", type=int, default=-1, help="attn_decode: warps per block of the kernel with the keys on the tile's rows (0: the other kernel; default: the engine's choice)")
     ap.add_argument("--shortest", type=int, default=0, help="attn_decode: lengths uniform in [shortest, context] instead of all equal")
+    ap.add_argument("--nodes", type=int, default=64, help="attn_tree: nodes of every tree, each below any one before it")
+    ap.add_argument("--beams", type=int, default=8)
+    ap.add_argument("--width", type=int, default=0, help="beam_select: candidates of a sequence (default: twice the beams)")
     ap.add_argument("--iters", type=int, default=20)
     ap.add_argument("--warmup", type=int, default=3)
     ap.add_argument("--pdl", action="store_true")
@@ -222,6 +226,35 @@ def main() -> int:
         out.update(shape=[B, S, H, G, K, V], delta=int(args.delta), us=round(us, 2), ns_per_token=round(us * 1e3 / S, 1),
                    gfma_per_s=round(fma / us / 1e3, 1), frac_fp32=round(fma / us * 1e6 / peak, 3),
                    gbs=round(nbytes / us / 1e3, 1), frac_hbm=round(nbytes / us / 1e3 / hbm, 3))
+    elif args.kernel == "attn_tree":
+        B, S, H, KV, hd, n = args.batch, args.context, args.heads, args.kv_heads, args.head_dim, args.nodes
+        import numpy as np
+        from ..engine.step import tree_facts
+        pages_per = (S + n + 63) // 64
+        n_sets = max(2, L2_BYTES * 2 // (B * pages_per * KV * 64 * hd * 2 * 2) + 1)
+        kc = torch.randn(n_sets * B * pages_per + 1, KV, 64, hd, device=dev, dtype=bf)
+        vc = torch.randn_like(kc)
+        tables = [(torch.arange(B * pages_per, dtype=torch.int32, device=dev).reshape(B, pages_per) + 1 + s * B * pages_per) for s in range(n_sets)]
+        draw = torch.Generator().manual_seed(0)
+        parents = [[-1] + [int(torch.randint(i, (1,), generator=draw)) for i in range(1, n)] for _ in range(B)]
+        masks = torch.from_numpy(np.concatenate([tree_facts(p, (n + 31) // 32)[0] for p in parents]).view(np.int32)).to(dev)
+        i32 = lambda x: torch.tensor(x, dtype=torch.int32, device=dev)
+        cu, slots, pos0 = i32([n * b for b in range(B + 1)]), i32(list(range(B))), i32([S] * B)
+        q, o = torch.randn(B * n, H * hd, device=dev, dtype=bf), torch.empty(B * n, H * hd, device=dev, dtype=bf)
+        us = _time(lambda i: ops.attention_tree(q, kc, vc, tables[i], cu, slots, pos0, masks, B, n, S + n, H, KV, hd, hd ** -0.5, o),
+                   n_sets, args.iters, args.warmup)
+        nbytes, flops = B * (S + n) * KV * hd * 2 * 2 + 2 * B * n * H * hd * 2, 4.0 * B * n * (S + n) * H * hd
+        out.update(shape=[B, n, S, H, KV, hd], us=round(us, 2), gbs=round(nbytes / us / 1e3, 1), frac_hbm=round(nbytes / us / 1e3 / hbm, 3),
+                   tflops=round(flops / us / 1e6, 1), frac_tensor=round(flops / us / 1e6 / tflops, 3))
+    elif args.kernel == "beam_select":
+        rows, width = args.batch * args.beams, args.width or 2 * args.beams
+        n_sets = max(2, L2_BYTES * 2 // (rows * args.n * 4) + 1)
+        logits = [torch.randn(rows, args.n, device=dev) for _ in range(n_sets)]
+        scores = -torch.rand(args.batch, args.beams, device=dev)
+        us = _time(lambda i: ops.beam_select(logits[i], scores, width), n_sets, args.iters, args.warmup)
+        nbytes = rows * args.n * 4
+        out.update(shape=[args.batch, args.beams, args.n], width=width, us=round(us, 2), gbs=round(nbytes / us / 1e3, 1),
+                   frac_hbm=round(nbytes / us / 1e3 / hbm, 3))
     elif args.kernel == "rmsnorm":
         x = torch.randn(args.m, args.k, device=dev)
         w = torch.ones(args.k, device=dev, dtype=bf)
