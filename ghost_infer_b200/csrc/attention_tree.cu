@@ -11,7 +11,9 @@
 // head's group, which share every key and value that is read) and a range of tiles of 64 keys (attention_tree.cuh).  Scores are a
 // register tile of R / 16 rows by 4 keys a thread, sums of values R / 16 rows by 4 numbers for every 64 of the head; a row's 16
 // threads are one half of a warp, so its maximum and sum need no barrier.
-// Bound: 32-bit multiply-adds (4 per query number, key and value) with many rows, the cache's bytes with few.
+// Bound: 32-bit multiply-adds (2 per query number and key) with many rows, the cache's bytes with few.  B200, 3 trees of 5 to 17
+// nodes behind 100 to 701 positions, 32 heads of 64 over 8: 20 us with the join (two tiles a block 30; breaks inside the inner loops
+// for rows that are not there 33; the body for 16 rows beside the one for 64 chosen by unit instead).
 #include <type_traits>
 
 #include "api.h"

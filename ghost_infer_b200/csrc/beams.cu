@@ -19,7 +19,8 @@
 // value and then place, no two are alike, and the bar rises every time.
 // A sum that is no number (a logit was none, was infinite, or too large to be scaled) sends the part through once more with every
 // logit looked at: what is no number counts as -inf.
-// Bound: the instructions, about ten a logit (half of them the sum's), next to the logits' bytes.
+// Bound: the instructions, about twenty a logit.  B200, 32 sequences of 8 beams over 128,256 tokens, 16
+// candidates: 38 us (3.4 TB/s) and 7 us of the join; one sequence of 4 beams 9.5 us in all.
 #include <math.h>
 
 #include "api.h"

@@ -8,7 +8,9 @@
 // overwrites what a later one reads; a thread that moves its column of 2 to 16 bytes of every accepted row in the path's order
 // needs nobody to wait for.
 // Every block repeats the walk over its sequence's nodes in shared memory (one warp, a round of the nodes per accepted one): that
-// costs less than a launch of its own that the moves would wait for.  Bound: latency; the moved rows' bytes for many sequences.
+// costs less than a launch of its own that the moves would wait for.  Bound: latency.  B200: one tree of 26 nodes, 28 layers, 4 us; 64
+// trees of up to 61 nodes 17 us for 35 MB (blocks of several columns a thread, so fewer walks: 16 us with 8 blocks an SM, 20 with 4, 28
+// with 2; it is the rows' trips to memory that take the time).
 #include "api.h"
 #include "common.cuh"
 #include "page_tensors.cuh"
