@@ -188,7 +188,9 @@ def cmd_run(o: Opts) -> None:
         from .kernels import ops
         ops.profile_start()
     if o.beams:
-        results = [r[0] for r in llm.beam_search(prompts, beams=o.beams, max_new=o.max_new, batch_size=batch)]
+        from .engine.beams import BeamResult
+        found = llm.beam_search(prompts, beams=o.beams, max_new=o.max_new, batch_size=batch)
+        results = [r[0] if r else BeamResult([], 0.0, 0.0, "stop") for r in found]      # (none: logits that are no numbers)
     elif o.draft:
         results = llm.generate_drafted(prompts, max_new=o.max_new, max_nodes=o.draft + 1, batch_size=batch)
     else:

@@ -6,6 +6,7 @@ one-token steps would have picked.  The decisions about ends are the reference's
 """
 from __future__ import annotations
 
+import time
 from dataclasses import dataclass
 from typing import Callable, Dict, List, Sequence, Tuple
 
@@ -13,6 +14,8 @@ from ..cache.pages import CacheFullError, pages_for
 from ..kernels import ops
 from .generate import GenerationResult, GenerationStats
 from .step import MAX_TREE_NODES, StepEntry, TreeEntry
+
+MAX_SEQS = 1024                # sequences of one step over trees (the tree attention's limit)
 
 # (tokens so far, most nodes) -> (tokens, parents): parents index the returned tokens, -1 continues the last token so far
 Drafter = Callable[[Sequence[int], int], Tuple[List[int], List[int]]]
@@ -34,7 +37,7 @@ class PromptLookup:
         for n in range(min(self.longest, len(tokens) - 1), 0, -1):
             suffix, found = tokens[-n:], 0
             for at in range(len(tokens) - n - 1, -1, -1):
-                if tokens[at:at + n] != suffix:
+                if tokens[at + n - 1] != suffix[-1] or tokens[at:at + n] != suffix:
                     continue
                 node = -1
                 for t in tokens[at + n:at + n + self.length]:
@@ -77,7 +80,7 @@ class DraftedLoop:
         first = 0
         while first < len(prompts):
             free, n = cache.free_pages, 0
-            while n < self.batch_size and first + n < len(prompts) and n < cache.slots.free_slots:
+            while n < min(self.batch_size, MAX_SEQS) and first + n < len(prompts) and n < cache.slots.free_slots:
                 need = pages_for(len(prompts[first + n]) + 1)
                 if need > free:
                     break
@@ -114,6 +117,7 @@ class DraftedLoop:
         engine, cache = self.engine, self.engine.cache
         slots: Dict[int, int] = {}
         self.stats.batches += 1
+        t0, t1 = time.perf_counter(), None
         try:
             for i in ids:
                 slots[i] = cache.open_slot()
@@ -126,6 +130,8 @@ class DraftedLoop:
             self.stats.prompt_tokens += sum(len(prompts[i]) for i in ids)
             live = [i for i, t in zip(ids, ops.sample(logits, 0.0, 0, 1.0).cpu().tolist())
                     if self._take(results[i], t, cache.length(slots[i]), max_new)]
+            t1 = time.perf_counter()                   # (the picks have been read back: the prompts are through)
+            self.stats.prompt_secs += t1 - t0
             while live:
                 entries = []
                 for i in live:
@@ -156,5 +162,7 @@ class DraftedLoop:
                         going.append(i)
                 live = going
         finally:
+            if t1 is not None:
+                self.stats.gen_secs += time.perf_counter() - t1
             for s in slots.values():
                 cache.close_slot(s)

@@ -274,3 +274,34 @@ def test_command_line_options():
         with pytest.raises(cli.UsageError):
             cli.cmd_run(cli.parse_opts(["m", "-p", "1"] + args))
     assert plain_walk([], [], []) == ([], -1)
+
+
+def test_a_search_that_finds_nothing_prints_an_empty_line(monkeypatch, capsys):
+    """Logits that are no numbers leave a beam search without results."""
+    class Llm:
+        last_stats = None
+
+        def beam_search(self, prompts, **kw):
+            return [[] for _ in prompts]
+    monkeypatch.setattr(cli, "_llm", lambda *a, **k: Llm())
+    cli.cmd_run(cli.parse_opts(["m", "-p", "1,2;3", "--beams", "2"]))
+    assert capsys.readouterr().out.split("\n")[:2] == ["", ""]
+
+
+def test_drafted_batches_are_no_larger_than_a_launch_takes():
+    class Slots:
+        free_slots = 5000
+
+    class Cache:
+        max_seq_len, free_pages, slots = 100, 5000, Slots()
+
+    class Engine:
+        cache = Cache()
+
+        def takes_trees(self):
+            return True
+    loop = DraftedLoop(Engine(), PromptLookup(), batch_size=3000)
+    taken = []
+    loop._run_batch = lambda prompts, results, ids, max_new: taken.append(len(ids))
+    loop.run([[1]] * 2500, 4)
+    assert taken == [1024, 1024, 452]

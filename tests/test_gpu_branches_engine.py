@@ -169,6 +169,15 @@ def test_drafted_generation_at_the_ends_of_context_and_pool(model_dirs, tiny_con
         assert [r.finish_reason for r in llm.generate_drafted(prompts, max_new=0)] == ["length"] * 2
 
 
+def test_drafted_generation_says_how_long_it_took(model_dirs, tiny_configs):
+    llm = gi.LLM(model_dirs("A", "float32"), dtype="float32", max_tokens=64 * 40)
+    prompts = [tokens_for(tiny_configs["A"], n, n) for n in (20, 3)]
+    llm.generate_drafted(prompts, max_new=9, batch_size=1, stop_token_ids=())
+    st = llm.last_stats
+    assert st.prompt_secs > 0 and st.gen_secs > 0
+    assert (st.prompt_tokens, st.gen_tokens, st.batches) == (23, 18, 2)
+
+
 # ---- beam search ------------------------------------------------------------------------------------------------------------
 def plain_beams(log_probs_of, prompt, beams, max_new, stop, width):
     """Beam search by the plain implementation: every beam's whole sequence is run again at every step."""
