@@ -201,7 +201,7 @@ attn_tree_kernel(const Shape sh, T* __restrict__ out, long ldo, const T* q, long
               v4[c] = c * 64 + tx * 4 < hp ? *reinterpret_cast<const float4*>(Vs + (j + w) * ld + c * 64 + tx * 4) : make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
             for (int i = 0; i < RT; ++i) {
-                    const float p = w == 0 ? p4[i].x : w == 1 ? p4[i].y : w == 2 ? p4[i].z : p4[i].w;
+              const float p = w == 0 ? p4[i].x : w == 1 ? p4[i].y : w == 2 ? p4[i].z : p4[i].w;
               if (decltype(look_twice)::value && p == 0.f) continue;
 #pragma unroll
               for (int c = 0; c < DCH; ++c) {

@@ -2,9 +2,10 @@
 
 The reference samples one continuation (src/main.rs:702-786).  Here a prompt is read once, its slot is forked into as many as
 there are beams (pages are shared, see `SequenceCache.fork`), and every step is: one token for all beams of all sequences, the
-2 x beams best of beams x vocabulary (`ops.beam_select`), the ones among them that end the sequence set aside, the others'
+2 x beams (or more) best of beams x vocabulary (`ops.beam_select`), the ones among them that end the sequence set aside, the others'
 first `beams` fed next after the cache has followed them (`SequenceCache.reorder`).  Twice as many candidates as beams leave
-enough that do not end: a beam has one stop token's worth of candidates for each of the stop tokens, of which the best counts.
+enough that do not end: a beam has a candidate that ends for each of the stop tokens.  More stop tokens ask for more candidates, as
+many as `ops.beam_select` gives (64); where all of those were ends, fewer beams would go on.
 """
 from __future__ import annotations
 

@@ -364,10 +364,9 @@ class Engine:
         return TreeStep(self.forward(ctx), ctx, list(entries))
 
     def commit_tree(self, tree: TreeStep, picks: torch.Tensor) -> List[List[int]]:
-        """Takes over what the picks (int32 [nodes] on the device, in the order of the logits' rows: the token chosen after each node)
-        agree with: from a tree's first
-        node on, the child whose token is the pick, as long as there is one.  The slots then hold the accepted tokens.
-        Returns, for every entry, the accepted nodes' tokens after the first, and behind them the pick after the last one."""
+        """Takes over what the picks (int32 [nodes] on the device, in the order of the logits' rows: the token chosen after each
+        node) agree with: from a tree's first node on, the child whose token is the pick, as long as there is one.  The slots then
+        hold the accepted tokens.  Returns, for every entry, the accepted nodes' tokens after the first, and behind them the pick after the last one."""
         from ..kernels import ops
         if tree.done:
             raise RuntimeError("this step has been committed already")
