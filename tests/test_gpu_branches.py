@@ -467,6 +467,58 @@ def test_tree_attention_graph_and_streams():
         assert all(torch.equal(t, want_b) for t in there) and all(torch.equal(t, want_a) for t in here)
 
 
+def test_a_run_of_them_with_launches_that_begin_early():
+    """Each reads what the one before it wrote; launched to begin before its predecessor has ended, eagerly and from a recording,
+    the run gives what it gives with every launch on its own."""
+    seqs, beams, vocab = 2, 4, 40000
+    sizes, pos0 = [20, 9], [300, 40]
+    case = TreeCase(sizes, pos0, 8, 2, 128, BF16, seed=31)
+    logits, first_scores = randn(seqs * beams, vocab, seed=32, scale=3.0), randn(seqs, beams, seed=33)
+    state0, slots = randn(seqs * beams, 4096, seed=34), i32([[3, 1, 0, 2], [6, 7, 5, 4]])
+    pages0 = randn(2, 12, 2, 64, 64, dtype=BF16, seed=35)
+    cu, seq_slots, at = i32([0, 20, 29]), i32([0, 1]), i32([70, 10])
+    table, node_parents = i32([[1, 2, 3], [4, 5, 6]]), i32(([-1] + list(range(19))) + [-1] + list(range(8)))
+    state, pages, out = state0.clone(), pages0.clone(), torch.zeros_like(case.run())
+
+    def run():
+        scores, parents, tokens = ops.beam_select(logits, first_scores, beams)
+        ops.reorder_states([state], slots, parents)
+        # the moved states choose which pages are copied, the beams' tokens which drafts hold
+        src = (state[:2, 0] > 0).int() + 1
+        ops.copy_pages([pages], src, i32_pages, i32_rows)
+        case.run(out=out)
+        picks = (tokens.view(-1)[0] + torch.zeros(29, dtype=torch.int32, device=DEV)).int()
+        path, counts, nexts = ops.tree_commit(picks, picks.clone(), node_parents, cu, seq_slots, at, 2, 20, [pages], table)
+        return [scores, parents, tokens, path, counts, nexts]
+
+    i32_pages, i32_rows = i32([4, 5]), i32([64, 33])
+
+    def fresh():
+        state.copy_(state0)
+        pages.copy_(pages0)
+        out.zero_()
+
+    was = ops.get_pdl()
+    try:
+        ops.set_pdl(False)
+        want = [t.clone() for t in run() + [state, pages, out]]
+        assert want[4].tolist() == [20, 9]                  # (every pick is every token: whole chains are accepted)
+        ops.set_pdl(True)
+        for _ in range(20):
+            fresh()
+            assert all(torch.equal(a, b) for a, b in zip(run() + [state, pages, out], want))
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            got = run()
+        for _ in range(20):
+            fresh()
+            graph.replay()
+            assert all(torch.equal(a, b) for a, b in zip(got + [state, pages, out], want))
+    finally:
+        ops.set_pdl(was)
+
+
 # ---- what is refused ----------------------------------------------------------------------------------------------------------
 def test_refusals():
     logits, scores = randn(4, 100), torch.zeros(2, 2, device=DEV)
