@@ -671,7 +671,8 @@ int gi_linear_state_keyed(float* o, const void* q, long ldq, const void* k, long
                           const int* seq_slots, int n_seqs, int heads, int K, int V, int n_tokens, void* stream);
 
 // Beam search's choice: of every sequence's beams x vocabulary the `width` (1 to 64) largest of score + log softmax(logits), compared
-// in 64 bits, in descending order; of equal ones the lowest beam's first, then the larger logit, then the lowest token.  logits: [seqs * beams] rows of `vocab`
+// in 64 bits, in descending order; of equal ones the lowest beam's first, then the larger logit, then the lowest token.  A row's log sum
+// is good to 3e-6, and equal rows have the same one wherever they lie and whatever else a call holds.  logits: [seqs * beams] rows of `vocab`
 // numbers (`dtype`, row stride ld), beams 1 to 64; scores float [seqs * beams].  A logit that is no number counts as -inf; a beam
 // whose logits are all -inf, hold a +inf, or whose score is not finite offers nothing.  Outputs [seqs][width]; where there is
 // nothing left: score -inf, parent and token -1.  scratch: gi_beam_select_scratch bytes, 16-byte aligned.

@@ -5,23 +5,33 @@
 // and the `width` largest of a sequence's beams x vocabulary are wanted in order; of equal ones the lowest beam's first, within a
 // beam the larger logit (64 bits may not tell two sums apart whose logits differ), then the lowest token.  One pass over
 // the logits does both halves: the sum of exponentials, and the `width` largest logits (within a row the logits' order is the
-// candidates').  A second kernel joins a sequence's rows: their log sums, then the `width` largest candidates of all lists,
-// compared in 64 bits, so that the order between two beams does not hang on the rounding of a sum.
+// candidates').  A second kernel joins a sequence's rows: their log sums, then the `width` largest candidates of all lists.
+//
+// A row's sum is made of pieces that its columns alone name: for every 1,024 of them (a warp's share of a tile) the largest logit
+// m and the sum of exp(x - m) in 32 bits, always by the same additions, joined in 64 bits in the pieces' order.  So equal rows have
+// equal sums, wherever they start in memory and whatever else the call holds, and their candidates tie as they should.  x - m is
+// taken before it is scaled: the error of a sum does not grow with the logits.  With d the mean of m - x under the row's
+// probabilities (at most ln V), a log sum is off by at most 2^-22 (an exponential) + 15 * 2^-24 (additions) + d * 2^-22.8 (the
+// exponents), under 3e-6 in the worst case; candidates of two beams that are further apart than that come in their true order.
+// Above a logit of 1e9 or so the 64 bits of a log sum, m + ln sum exp(x - m), are the coarser ones.
 //
 // The rows are cut into tiles of 8,192 logits; a block takes an equal range of the tiles of all rows, so that any number of
-// rows keeps all SMs busy, and leaves one part (sum, list) for every row it meets.  Tiles come through a ring in shared memory
-// (a thread reads back the pieces it asked for itself), which keeps 96 KB an SM under way with few registers; with the next
-// tile in registers instead, the kernel spilled and took twice as long.
+// rows keeps all SMs busy, and leaves one list for every row it meets.  Tiles come through a ring in shared memory, which keeps
+// 96 KB an SM under way with few registers; with the next tile in registers instead, the kernel spilled and took twice as
+// long.  A warp fetches its columns of a tile in the aligned 16-byte pieces that hold them (of a row that starts between two
+// boundaries one more for every 32) and reads them by column.
 // What enters a part's list must reach a bar that at least `width` of the part's logits reach.  The first bar is the smallest of
 // the warps' k-th largest lane maxima in the part's first tile, k = ceil(width / warps).  After the part's tiles 1, 4, 16, ... the list
 // is cut down to its `width` best and the bar raised to the last of them: each step then adds about 3 `width` entries.  A
 // list that overflows all the same (equal logits) raises the bar and the part is gone through again: entries are ordered by
 // value and then place, no two are alike, and the bar rises every time.
-// A sum that is no number (a logit was none, was infinite, or too large to be scaled) sends the part through once more with every
-// logit looked at: what is no number counts as -inf.
-// Bound: the instructions, about twenty a logit.  B200, 32 sequences of 8 beams over 128,256 tokens, 16
-// candidates: 38 us (3.4 TB/s) and 7 us of the join; one sequence of 4 beams 9.5 us in all.
+// A piece whose sum is no number (a logit was none, or infinite) is added up once more with what is no number as -inf.
+// Bound: neither the memory (41 % of its rate) nor the issue slots (20 instructions a logit would fill them for 18 us), but what 20
+// warps an SM cannot hide: fixed latencies, the barriers around the lists, SMs that have two blocks and not three.  B200, 32
+// sequences of 8 beams over 128,256 tokens, 16 candidates: 43 us in all, the join a few of them; one sequence of 4 beams 9.4 us.
 #include <math.h>
+
+#include <type_traits>
 
 #include "api.h"
 #include "common.cuh"
@@ -35,6 +45,7 @@ constexpr int THREADS = 256, WARPS = THREADS / 32;
 constexpr int MAX_WIDTH = 64, MAX_BEAMS = 64;
 constexpr int CAP = 512;                    // entries of a part's list
 constexpr int NUMBERS = 32, STAGES = 2;     // numbers of a tile that a thread takes; tiles of the ring
+constexpr int TILE = THREADS * NUMBERS;
 
 // Order of floats as order of unsigned numbers; -inf gives the smallest key that occurs.
 __device__ __forceinline__ unsigned order_key(float v) {
@@ -51,6 +62,15 @@ __device__ __forceinline__ float ex2(float x) {
   return y;
 }
 constexpr float LOG2E = 1.4426950408889634f;
+
+// exp(x + shift) of two numbers; the additions and the products of both are one instruction each.
+__device__ __forceinline__ float2 exp2_of(float a, float b, float2 shift) {
+  float2 d;
+  asm("{\n\t.reg .b64 a, s, d, l;\n\tmov.b64 a, {%2, %3};\n\tmov.b64 s, {%4, %5};\n\tmov.b64 l, {%6, %6};\n\tadd.rn.f32x2 d, a, s;\n\t"
+      "mul.rn.f32x2 d, d, l;\n\tmov.b64 {%0, %1}, d;\n\t}"
+      : "=f"(d.x), "=f"(d.y) : "f"(a), "f"(b), "f"(shift.x), "f"(shift.y), "f"(LOG2E));
+  return make_float2(ex2(d.x), ex2(d.y));
+}
 
 // A 16-byte piece of a row as it is fetched, and its numbers.
 template <typename T> struct Piece;
@@ -131,35 +151,19 @@ __device__ __forceinline__ void cut_down(Lists& s, int width) {
   __syncthreads();
 }
 
-// part_stat [row][parts]: (reference, sum of exp(x - reference)); part_key [row][parts][width]: logits in descending order as
-// (order of the value, ~token), 0 where there are no more.
+// row_sum [row][tile][warp]: (m, sum of exp(x - m)) of the warp's columns; part_key [row][parts][width]: logits in descending
+// order as (order of the value, ~token), 0 where there are no more.
 template <typename T>
 __global__ void __launch_bounds__(THREADS, 3)
-beam_rows_kernel(const T* logits, long ld, int vocab, int rows, Cut cut, int width, double2* __restrict__ part_stat, u64* __restrict__ part_key) {
-  constexpr int N = Piece<T>::N, VPT = NUMBERS / N;
+beam_rows_kernel(const T* logits, long ld, int vocab, int rows, Cut cut, int width, float2* __restrict__ row_sum, u64* __restrict__ part_key) {
+  constexpr int N = Piece<T>::N, VPT = NUMBERS / N, WARP_PIECES = 33;
   extern __shared__ __align__(16) unsigned char smem[];
-  uint4* ring = (uint4*)smem;                        // [STAGES][VPT][THREADS]
+  uint4* ring = (uint4*)smem;                        // [STAGES][VPT][WARPS][33 pieces]
   __shared__ Lists s;
-  __shared__ float s_ref[WARPS];
-  __shared__ double s_sum[WARPS];
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   gi::pdl_prologue();
   const long lo = (long)blockIdx.x * cut.per, hi = min((long)rows * cut.tiles_row, lo + cut.per);
 
-  // A row's 16-byte pieces lie between the first 16-byte boundary in it and the last; the few numbers before and after them go
-  // with its first tile.
-  struct Row {
-    const T* x;
-    int lead, pieces, tail;
-  };
-  auto row_of = [&](int row) {
-    Row r;
-    r.x = logits + (size_t)row * ld;
-    r.lead = min(vocab, (int)((16 - ((uintptr_t)r.x & 15)) & 15) / (int)sizeof(T));
-    r.pieces = (vocab - r.lead) / N;
-    r.tail = vocab - r.lead - r.pieces * N;
-    return r;
-  };
   // a place in the list of tiles, counted up without divisions
   struct Place {
     int left, row, tile, stage;                      // tiles up to the end of the block's range
@@ -172,15 +176,21 @@ beam_rows_kernel(const T* logits, long ld, int vocab, int rows, Cut cut, int wid
   Place here;
   here.left = (int)max(0L, hi - lo), here.row = (int)(lo / cut.tiles_row), here.tile = (int)(lo - (long)here.row * cut.tiles_row), here.stage = 0;
   Place asked = here;                                // the next tile to ask for
+  // A row's numbers i N ... i N + N - 1 lie in piece i of 16 bytes from the last boundary before the row on, and where the row starts
+  // behind that boundary, in piece i + 1.  Nothing past the row's last byte is fetched; what is fetched in front of its first one
+  // lies in the same 16 bytes as that.
   auto ask = [&]() {
     if (asked.left > 0) {
-      const Row r = row_of(asked.row);
-      const uint4* body = reinterpret_cast<const uint4*>(r.x + r.lead);
-      uint4* to = ring + asked.stage * VPT * THREADS + tid;
+      const uintptr_t first = (uintptr_t)(logits + (size_t)asked.row * ld), from = first & ~(uintptr_t)15, end = first + (size_t)vocab * sizeof(T);
+      uint4* to = ring + (asked.stage * VPT * WARPS + warp) * WARP_PIECES;
 #pragma unroll
       for (int i = 0; i < VPT; ++i) {
-        const int at = (asked.tile * VPT + i) * THREADS + tid;
-        if (at < r.pieces) gi::cp_async_16(gi::smem_u32(to + i * THREADS), body + at, 16);
+        const uintptr_t at = from + ((size_t)(asked.tile * VPT + i) * THREADS + tid) * 16;
+        if (at < end) gi::cp_async_16(gi::smem_u32(to + i * WARPS * WARP_PIECES + lane), (const void*)at, (int)min(end - at, (uintptr_t)16));
+      }
+      if (from != first && lane < VPT) {              // a lane each: the piece behind the warp's last one
+        const uintptr_t at = from + ((size_t)(asked.tile * VPT + lane) * THREADS + warp * 32 + 32) * 16;
+        if (at < end) gi::cp_async_16(gi::smem_u32(to + lane * WARPS * WARP_PIECES + 32), (const void*)at, (int)min(end - at, (uintptr_t)16));
       }
     }
     asked.next(cut.tiles_row);
@@ -190,38 +200,42 @@ beam_rows_kernel(const T* logits, long ld, int vocab, int rows, Cut cut, int wid
   for (int i = 0; i < STAGES - 1; ++i) ask();
 
   Place part = here;                                 // the part's first tile
-  int summed = here.left;                            // the sums hold every tile with more than that many left
   int next_cut = 1;                                  // tiles of the part after which its list is cut down
-  bool wild = false;                                 // a maximum of this thread's was too large to be scaled
-  float ref = 0.f, sum = 0.f;                        // of this thread's numbers: sum of 2^(x log2 e - ref)
-  bool keep_bar = false, careful = false;            // a part that is gone through again, and what for
+  bool keep_bar = false;                             // the part is gone through again
   while (here.left > 0) {
     const int row = here.row, tile = here.tile;
-    const Row r = row_of(row);
+    __syncwarp();                                    // (a warp's lanes read one another's pieces)
     ask();
     gi::cp_async_wait<STAGES - 1>();
-    float x[VPT * N + 1];
-    const uint4* from = ring + here.stage * VPT * THREADS + tid;
+    __syncwarp();
+    const unsigned off = (unsigned)(uintptr_t)(logits + (size_t)row * ld) & 15u;
+    const unsigned char* from = (const unsigned char*)(ring + (here.stage * VPT * WARPS + warp) * WARP_PIECES + lane) + off;
+    constexpr int STEP = WARPS * WARP_PIECES * 16;   // bytes from a thread's piece to its next one
+    float x[NUMBERS];
+    if (off == 0) {
 #pragma unroll
-    for (int i = 0; i < VPT; ++i) Piece<T>::numbers(from[i * THREADS], x + i * N);
-    if ((tile + 1) * VPT * THREADS > r.pieces) {
+      for (int i = 0; i < VPT; ++i) Piece<T>::numbers(*reinterpret_cast<const uint4*>(from + i * STEP), x + i * N);
+    } else {
+      const unsigned turn = 8 * (off & 3u);           // 16-bit numbers that start in the middle of a word
 #pragma unroll
-      for (int i = 0; i < VPT; ++i)
-        if ((tile * VPT + i) * THREADS + tid >= r.pieces) {
-#pragma unroll
-          for (int e = 0; e < N; ++e) x[i * N + e] = -INFINITY;
-        }
+      for (int i = 0; i < VPT; ++i) {
+        const unsigned* w = reinterpret_cast<const unsigned*>(from - (off & 3u) + i * STEP);
+        uint4 v;
+        if (sizeof(T) == 4 || turn == 0) v = make_uint4(w[0], w[1], w[2], w[3]);
+        else v = make_uint4(__funnelshift_r(w[0], w[1], turn), __funnelshift_r(w[1], w[2], turn), __funnelshift_r(w[2], w[3], turn), __funnelshift_r(w[3], w[4], turn));
+        Piece<T>::numbers(v, x + i * N);
+      }
     }
-    const int loose_at = tid < r.lead ? tid : vocab - r.tail + (tid - r.lead);
-    x[NUMBERS] = tile == 0 && tid < r.lead + r.tail ? gi::ldf(r.x + loose_at) : -INFINITY;
-    if (__builtin_expect(careful, false)) {
+    const int token0 = (tile * VPT * THREADS + tid) * N;         // piece i's first token: THREADS * N further each
+    if ((tile + 1) * (long)TILE > vocab) {
 #pragma unroll
-      for (int i = 0; i <= NUMBERS; ++i) x[i] = fmaxf(x[i], -INFINITY);
+      for (int i = 0; i < NUMBERS; ++i)
+        if (token0 + i / N * THREADS * N + i % N >= vocab) x[i] = -INFINITY;
     }
-    float tops[2] = {x[NUMBERS], -INFINITY};           // (a maximum passes over what is no number)
+    float tops[2] = {-INFINITY, -INFINITY};           // (a maximum passes over what is no number)
 #pragma unroll
     for (int i = 0; i < NUMBERS; ++i) tops[i & 1] = fmaxf(tops[i & 1], x[i]);
-    const float mine = fmaxf(fmaxf(tops[0], tops[1]), -INFINITY);
+    const float mine = fmaxf(tops[0], tops[1]);
 
     const bool first = here.left == part.left;
     if (first) {
@@ -232,44 +246,41 @@ beam_rows_kernel(const T* logits, long ld, int vocab, int rows, Cut cut, int wid
         if (!keep_bar) s.bar = (u64)bar << 32;
       }
       next_cut = 1;
-      if (summed == here.left) ref = 0.f, sum = 0.f, wild = false;
       __syncthreads();
     }
-    if (summed == here.left) {
-      // a thread's reference moves up with its maximum
-      if (mine > -INFINITY) {
-        // (scaled, unless it is too large for that: those parts are gone through carefully, with the reference itself)
-        const float top = careful ? mine : mine * LOG2E;
-        wild |= !(fabsf(top) < INFINITY);
-        if (top > ref || sum == 0.f) {
-          sum = sum == 0.f ? 0.f : sum * ex2(careful ? (ref - top) * LOG2E : ref - top);
-          ref = top;
-        }
+    const float m = key_value(__reduce_max_sync(0xffffffffu, order_key(mine)));
+    float sum = 0.f;
+    if (m > -INFINITY) {
+      const float2 shift = make_float2(-m, -m);
+      auto add_up = [&](auto look) {
         float more[4] = {0.f, 0.f, 0.f, 0.f};
-        if (__builtin_expect(careful, false)) {
 #pragma unroll
-          for (int i = 0; i <= NUMBERS; ++i) more[i & 3] += ex2((x[i] - ref) * LOG2E);
-        } else {
-#pragma unroll
-          for (int i = 0; i <= NUMBERS; ++i) more[i & 3] += ex2(fmaf(x[i], LOG2E, -ref));
+        for (int i = 0; i < NUMBERS; i += 2) {
+          const float2 e = exp2_of(decltype(look)::value ? fmaxf(x[i], -INFINITY) : x[i], decltype(look)::value ? fmaxf(x[i + 1], -INFINITY) : x[i + 1], shift);
+          more[i & 3] += e.x, more[(i & 3) + 1] += e.y;
         }
-        sum += (more[0] + more[1]) + (more[2] + more[3]);
-      }
-      --summed;
+        sum = (more[0] + more[1]) + (more[2] + more[3]);
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+      };
+      add_up(std::false_type());
+      if (__builtin_expect(!(sum < INFINITY), false)) add_up(std::true_type());      // (with m = +inf the sum stays none)
     }
+    if (lane == 0) row_sum[((size_t)row * cut.tiles_row + tile) * WARPS + warp] = make_float2(m, sum);
+
     const u64 bar = s.bar;
     const float bar_value = fmaxf(key_value((unsigned)(bar >> 32)), -3.402823466e38f);      // (-inf is nobody's candidate)
     if (mine >= bar_value) {
-      // which of the thread's numbers reach it, and one after the other from where they lie (33 copies of what follows, one for every
+      // which of the thread's numbers reach it, and one after the other from where they lie (32 copies of what follows, one for every
       // register, took more time to fetch than to execute)
-      u64 hits = 0;
+      unsigned hits = 0;
 #pragma unroll
-      for (int i = 0; i <= NUMBERS; ++i) hits |= x[i] >= bar_value ? (u64)1 << i : 0;
+      for (int i = 0; i < NUMBERS; ++i) hits |= x[i] >= bar_value ? 1u << i : 0;
       while (hits != 0) {
-        const int i = __ffsll((long long)hits) - 1;
+        const int i = __ffs(hits) - 1;
         hits &= hits - 1;
-        const float v = i < NUMBERS ? gi::ldf(reinterpret_cast<const T*>(from + i / N * THREADS) + i % N) : gi::ldf(r.x + loose_at);
-        const u64 own = entry_of(v, i < NUMBERS ? r.lead + ((tile * VPT + i / N) * THREADS + tid) * N + i % N : loose_at);
+        const float v = gi::ldf(reinterpret_cast<const T*>(from + i / N * STEP) + i % N);
+        const u64 own = entry_of(v, token0 + i / N * THREADS * N + i % N);
         if (own >= bar) {
           const int to = atomicAdd(&s.count, 1);
           if (to < CAP) s.list[to] = own;
@@ -286,6 +297,7 @@ beam_rows_kernel(const T* logits, long ld, int vocab, int rows, Cut cut, int wid
     if (over) {
       // the bar is the `width`-th best of what the list had room for: once more from the part's first tile
       gi::cp_async_wait<0>();
+      __syncwarp();
       here = asked = part;
 #pragma unroll
       for (int i = 0; i < STAGES - 1; ++i) ask();
@@ -293,35 +305,10 @@ beam_rows_kernel(const T* logits, long ld, int vocab, int rows, Cut cut, int wid
       continue;
     }
     if (!last) continue;
-    // the part's sum, in 64 bits over the threads, above the largest reference
-    const float own_ref = sum != 0.f ? ref : -INFINITY;
-    float top_ref = gi::warp_max(own_ref);
-    if (lane == 0) s_ref[warp] = top_ref;
-    const bool none = __syncthreads_or(wild || !(fabsf(sum) < INFINITY));
-    if (none && !careful) {
-      careful = keep_bar = true;                       // (the bar that the list ended with is reached by `width` logits)
-      summed = part.left;
-      gi::cp_async_wait<0>();
-      here = asked = part;
-#pragma unroll
-      for (int i = 0; i < STAGES - 1; ++i) ask();
-      continue;
-    }
-#pragma unroll
-    for (int w = 0; w < WARPS; ++w) top_ref = fmaxf(top_ref, s_ref[w]);
-    double total = sum != 0.f ? (double)sum * (double)ex2(careful ? (own_ref - top_ref) * LOG2E : own_ref - top_ref) : 0.0;
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) total += __shfl_xor_sync(0xffffffffu, total, o);
-    if (lane == 0) s_sum[warp] = total;
     const size_t out = (size_t)row * cut.parts + (blockIdx.x - cut.first_block(row));
     for (int i = tid; i < width; i += THREADS) part_key[out * width + i] = i < s.count ? s.list[i] : 0;
     __syncthreads();
-    if (tid == 0) {
-      double t = 0.0;
-      for (int w = 0; w < WARPS; ++w) t += s_sum[w];
-      part_stat[out] = make_double2(careful ? (double)top_ref : (double)top_ref * 0.69314718055994530942, t);
-    }
-    keep_bar = careful = false;
+    keep_bar = false;
     part = here;
   }
   gi::cp_async_wait<0>();
@@ -347,7 +334,7 @@ __device__ __forceinline__ u64 order_key(double v) {
 // side: for a bar that `width` of them reach (as in the rows' first tiles, on the upper halves of the candidates' keys), and for
 // those that reach it, which are put in order by counting.
 __global__ void __launch_bounds__(THREADS)
-beam_join_kernel(const float* scores, const double2* part_stat, const u64* part_key, int beams, Cut cut, int width,
+beam_join_kernel(const float* scores, const float2* row_sum, const u64* part_key, int beams, Cut cut, int width,
                  float* __restrict__ out_scores, int* __restrict__ out_parents, int* __restrict__ out_tokens) {
   constexpr int AHEAD = 4;
   __shared__ double s_base[MAX_BEAMS];
@@ -384,15 +371,22 @@ beam_join_kernel(const float* scores, const double2* part_stat, const u64* part_
     const int e = place_of(q);
     ahead[q] = e < entries ? key_at(e, beam_ahead[q]) : 0;
   }
-  // a row's log sum: a warp to a row, a lane to a part
+  // a row's log sum: a warp to a row, a lane to every 32nd piece of it
+  const int pieces = cut.tiles_row * WARPS;
   for (int j = warp; j < beams; j += WARPS) {
-    const double2* st = part_stat + ((size_t)seq * beams + j) * parts;
+    const float2* st = row_sum + ((size_t)seq * beams + j) * pieces;
     const double score = (double)scores[(size_t)seq * beams + j];
     double top = -INFINITY, sum = 0.0;
-    for (int p = lane; p < s_parts[j]; p += 32) {
-      const double2 v = st[p];
-      const double both = fmax(top, v.x);
-      if (both > -INFINITY) sum = (top > -INFINITY ? sum * exp(top - both) : 0.0) + (v.x > -INFINITY ? v.y * exp(v.x - both) : v.y);
+    for (int p0 = lane; p0 < pieces; p0 += 32 * AHEAD) {
+      float2 v[AHEAD];
+#pragma unroll
+      for (int k = 0; k < AHEAD; ++k) v[k] = p0 + 32 * k < pieces ? st[p0 + 32 * k] : make_float2(-INFINITY, 0.f);
+      double both = top;
+#pragma unroll
+      for (int k = 0; k < AHEAD; ++k) both = fmax(both, (double)v[k].x);
+      if (top > -INFINITY) sum *= exp(top - both);
+#pragma unroll
+      for (int k = 0; k < AHEAD; ++k) sum += v[k].x > -INFINITY ? (double)v[k].y * exp((double)v[k].x - both) : 0.0;
       top = both;
     }
     double both = top;
@@ -496,12 +490,11 @@ struct Plan {
   int blocks;
 };
 
-template <typename T> constexpr int SMEM_RING = STAGES * THREADS * NUMBERS * (int)sizeof(T);
+template <typename T> constexpr int SMEM_RING = STAGES * (NUMBERS / Piece<T>::N) * WARPS * 33 * 16;
 
 Plan plan_of(int rows, int vocab) {
-  const int tile = THREADS * NUMBERS;
   Plan p;
-  p.cut.tiles_row = (vocab + tile - 1) / tile;
+  p.cut.tiles_row = (vocab + TILE - 1) / TILE;
   const long slots = 3L * gi::sm_count(), total = (long)rows * p.cut.tiles_row;
   p.cut.per = (int)((total + slots - 1) / slots);
   p.blocks = (int)((total + p.cut.per - 1) / p.cut.per);
@@ -510,7 +503,7 @@ Plan plan_of(int rows, int vocab) {
 }
 
 template <typename T>
-int launch_rows(const T* logits, long ld, int vocab, int rows, const Plan& p, int width, double2* stat, u64* key, cudaStream_t s) {
+int launch_rows(const T* logits, long ld, int vocab, int rows, const Plan& p, int width, float2* sums, u64* key, cudaStream_t s) {
   auto kern = beam_rows_kernel<T>;
   static bool configured[gi::MAX_DEVICES_SEEN] = {false};
   int dev;
@@ -519,14 +512,15 @@ int launch_rows(const T* logits, long ld, int vocab, int rows, const Plan& p, in
     if (e != cudaSuccess) return gi::fail(GI_ERR_CUDA, "beam selection: %s", cudaGetErrorString(e));
     if (dev >= 0) configured[dev] = true;
   }
-  return gi::check(gi::launch(kern, dim3(p.blocks), dim3(THREADS), SMEM_RING<T>, s, logits, ld, vocab, rows, p.cut, width, stat, key), "beam selection");
+  return gi::check(gi::launch(kern, dim3(p.blocks), dim3(THREADS), SMEM_RING<T>, s, logits, ld, vocab, rows, p.cut, width, sums, key), "beam selection");
 }
 
 }  // namespace
 
 extern "C" long gi_beam_select_scratch(int rows, int vocab, int width) {
   if (rows <= 0 || vocab <= 0 || width <= 0) return 0;
-  return (long)rows * plan_of(rows, vocab).cut.parts * (16 + 8L * width);
+  const Plan p = plan_of(rows, vocab);
+  return (long)rows * (p.cut.tiles_row * (8L * WARPS) + p.cut.parts * (8L * width));
 }
 
 extern "C" int gi_beam_select(float* out_scores, int* out_parents, int* out_tokens, const void* logits, int dtype, long ld, const float* scores,
@@ -543,12 +537,12 @@ extern "C" int gi_beam_select(float* out_scores, int* out_parents, int* out_toke
   if (scratch_bytes < gi_beam_select_scratch(rows, vocab, width) || ((uintptr_t)scratch & 15))
     return gi::fail(GI_ERR_ARG, "beam selection: the scratch memory is too small or not aligned");
   if ((long)beams * p.cut.parts * width > 0x3fffffffL) return gi::fail(GI_ERR_UNSUPPORTED, "beam selection: %d beams in %d parts each", beams, p.cut.parts);
-  double2* stat = (double2*)scratch;
-  u64* key = (u64*)(stat + (size_t)rows * p.cut.parts);
+  float2* sums = (float2*)scratch;
+  u64* key = (u64*)(sums + (size_t)rows * p.cut.tiles_row * WARPS);
   cudaStream_t s = (cudaStream_t)stream;
   int rc = GI_OK;
-  GI_DISPATCH_DTYPE(dtype, T, rc = launch_rows((const T*)logits, ld, vocab, rows, p, width, stat, key, s));
+  GI_DISPATCH_DTYPE(dtype, T, rc = launch_rows((const T*)logits, ld, vocab, rows, p, width, sums, key, s));
   if (rc != GI_OK) return rc;
-  return gi::check(gi::launch(beam_join_kernel, dim3(seqs), dim3(THREADS), 0, s, scores, stat, key, beams, p.cut, width, out_scores,
+  return gi::check(gi::launch(beam_join_kernel, dim3(seqs), dim3(THREADS), 0, s, scores, sums, key, beams, p.cut, width, out_scores,
                               out_parents, out_tokens), "beam selection (join)");
 }

@@ -2927,9 +2927,11 @@ def _i32_rows(t: torch.Tensor, what: str) -> int:
 
 def beam_select(logits: torch.Tensor, scores: torch.Tensor, width: int):
     """Beam search's choice: of every sequence's beams x vocabulary the `width` largest of score + log softmax(logits), in
-    descending order, compared in 64 bits; of equal ones the lowest beam's first, then the larger logit, then the lowest token.
-    logits [sequences * beams, vocab] (float32 or bfloat16, contiguous rows), scores float32 [sequences, beams].  Returns scores float32, parents int32 (the
-    beam that goes on) and tokens int32, each [sequences, width]; where no candidate is left: -inf, -1, -1.  A logit that is
+    descending order, compared in 64 bits; of equal ones the lowest beam's first, then the larger logit, then the lowest token.  A row's
+    log sum is good to 3e-6 whatever the size of its logits (beside one of 1e9 the 64 bits hold 1e-7 of it, less beyond), and equal rows
+    have the same one, so that equal beams tie.  logits [sequences * beams, vocab] (float32 or bfloat16, contiguous rows), scores
+    float32 [sequences, beams].  Returns scores float32, parents int32 (the beam that goes on) and tokens int32, each [sequences,
+    width]; where no candidate is left: -inf, -1, -1.  A logit that is
     no number counts as -inf; a beam whose logits are all -inf or hold a +inf, or whose score is not finite, offers nothing."""
     lib = _bind()
     stream = _on_here("beam selection", logits, scores)

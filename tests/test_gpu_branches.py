@@ -108,6 +108,72 @@ def test_beam_select_graph_and_stream():
     assert torch.equal(got[2], ops.beam_select(logits, scores, 8)[2])
 
 
+def check_beams_closely(logits, scores, width, off):
+    """`off`: what the log sum may be off by; added to a large logit in 64 bits it may become the number next to the plain one's."""
+    got = [t.cpu().numpy() for t in ops.beam_select(logits, scores, width)]
+    want = plain_beam_select(logits.cpu().double().numpy(), scores.cpu().double().numpy(), width)
+    assert (got[1] == want[1]).all() and (got[2] == want[2]).all()
+    assert (np.abs(got[0].astype(np.float64) - want[0]) <= off + 2.0 ** -52 * float(logits.abs().max()) + 2.0 ** -24 * np.abs(want[0])).all()
+
+
+@pytest.mark.parametrize("shift", [-1e6, -1e4, -1e3, -100.0, 0.0, 100.0, 1e3, 1e4, 1e6])
+def test_beam_select_log_sums_of_rows_far_from_zero(shift):
+    """The error of a log sum does not grow with the logits.  A number's exponent is rounded twice and scaled by a 32-bit log2(e)
+    (2^-22.8 of it in all), under a row's probabilities at most ln 40,000 = 10.6 of it; an exponential is good to 2^-22, 15 additions lie
+    on a number's way: below 2.6e-6."""
+    logits = randn(4, 40000, seed=int(abs(shift)), scale=3.0) + shift
+    # (two beams' candidates may lie nearer to each other than that: one beam a sequence)
+    check_beams_closely(logits, randn(4, 1, seed=2), 16, 2.6e-6)
+
+
+@pytest.mark.parametrize("top", [20.0, 50.0, 120.0, 1020.0, 10020.0, -3e5])
+def test_beam_select_sure_tokens(top):
+    """Next to a token that has all of the probability the others' sum is nothing: no error but the result's own rounding, and no
+    log probability above zero."""
+    logits = randn(3, 20000, seed=4) - 200.0 + top
+    logits[:, 777] = top
+    scores = torch.zeros(3, 1, device=DEV)
+    check_beams_closely(logits, scores, 5, 1e-7)
+    assert (ops.beam_select(logits, scores, 1)[0] == 0).all()
+
+
+@pytest.mark.parametrize("value", [-4e9, -6e9, -1e9, -1e11, -1e12, -1e15, -1e25, -1e30, 1e9, 1e25])
+def test_beam_select_rows_of_one_finite_value(value):
+    """A row that a mask filled throughout with a large finite number still has tokens, each as likely as another."""
+    check_beams_closely(torch.full((2, 9000), value, device=DEV), torch.tensor([[-1.0], [0.5]], device=DEV), 6, 2.6e-6)
+    mixed = torch.full((2, 9000), value, device=DEV)
+    mixed[0, 4000:4003] = abs(value)
+    check_beams_closely(mixed, torch.tensor([[-1.0], [0.5]], device=DEV), 6, 2.6e-6)
+
+
+@pytest.mark.parametrize("dtype,seqs,beams,vocab", [(F32, 1, 8, 32003), (F32, 1, 2, 32003), (F32, 8, 8, 128256), (F32, 20, 5, 70001), (BF16, 2, 8, 32003), (BF16, 30, 4, 50257)])
+def test_beam_select_equal_beams_tie_wherever_their_rows_lie(dtype, seqs, beams, vocab):
+    """Rows that start on different boundaries, and are cut at different places by the calls' many blocks, have the same sum."""
+    row = randn(1, vocab, dtype=dtype, seed=vocab + beams, scale=3.0)
+    logits = row.expand(seqs * beams, -1).contiguous()
+    got = ops.beam_select(logits, torch.full((seqs, beams), -2.5, device=DEV), beams)
+    best = torch.arange(vocab, device=DEV)[row[0] == row[0].max()].tolist()
+    want = [(j, t) for j in range(beams) for t in best][:beams]
+    assert got[1].tolist() == [[j for j, _ in want]] * seqs and got[2].tolist() == [[t for _, t in want]] * seqs
+    assert (got[0] == got[0][0, 0]).all()
+
+
+def test_beam_select_does_not_depend_on_the_rest_of_the_call():
+    logits, scores = randn(80, 65000, seed=6, scale=3.0), randn(20, 4, seed=7)
+    together = ops.beam_select(logits, scores, 12)
+    for s in (0, 7, 19):
+        alone = ops.beam_select(logits[4 * s:4 * s + 4], scores[s:s + 1].contiguous(), 12)
+        assert all(torch.equal(a[s:s + 1], b) for a, b in zip(together, alone))
+    for dtype, vocab in ((F32, 65003), (BF16, 65003)):
+        rows = randn(4, vocab, dtype=dtype, seed=8, scale=3.0)
+        want = ops.beam_select(rows, scores[:1].contiguous(), 20)
+        for shift in range(1, 9):
+            wide = torch.full((4, vocab + 16 + shift), 60.0, dtype=dtype, device=DEV)      # (what lies around a row is larger than all of it)
+            wide[:, shift:shift + vocab] = rows
+            got = ops.beam_select(wide[:, shift:shift + vocab], scores[:1].contiguous(), 20)
+            assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
 # ---- states and pages -------------------------------------------------------------------------------------------------------
 @pytest.mark.parametrize("beams", [1, 2, 4, 5, 8, 9, 16, 17, 40, 41, 64])
 @pytest.mark.parametrize("kind", ["float", "mixed"])
