@@ -384,21 +384,18 @@ class SequenceCache:
     def truncate(self, slot: int, pos: int) -> int:
         """Rewinds a slot to `pos` tokens (src/model.rs:799-821: lowering the position is enough for
         attention caches).  Returns the length actually reached: fixed-size state and released window
-        pages cannot be rewound, so with those the slot stays where it is."""
+        pages cannot be rewound, so with those the slot stays where it is.  Pages past that length go back."""
         cur = self.lengths[slot]
-        if pos >= cur:
-            return cur
-        if self._state or self._block_state or any(g.request.kind in ("window", "chunk") and g.first_live[slot] * PAGE_TOKENS > 0 for g in self._groups):
-            return cur
+        if pos < cur and not (self._state or self._block_state or any(g.request.kind in ("window", "chunk") and g.first_live[slot] * PAGE_TOKENS > 0 for g in self._groups)):
+            cur = self.lengths[slot] = pos
+        keep = pages_for(cur)
         for g in self._groups:
-            keep = pages_for(pos)
             pages = g.pages[slot]
             if len(pages) > keep:
                 g.pool.give_back(pages[keep:])
                 g.table_host[slot, keep:len(pages)] = 0
                 del pages[keep:]
-        self.lengths[slot] = pos
-        return pos
+        return cur
 
     # ---- device side ------------------------------------------------------------------------
     def sync_tables(self) -> None:

@@ -346,7 +346,8 @@ class Engine:
 
     def step_tree(self, entries: Sequence[TreeEntry]) -> TreeStep:
         """Runs every slot's tree of drafted tokens after what the slot holds.  The slots' lengths do not change before
-        `commit_tree`; a step that is not committed leaves nothing behind."""
+        `commit_tree`; a step that is not committed leaves nothing behind but pages that its slots will use next
+        (`SequenceCache.truncate` to a slot's own length gives them back)."""
         self._validate_trees(entries)
         self.cache.reserve([(e.slot, self.cache.length(e.slot) + len(e.tokens)) for e in entries])
         self.cache.sync_tables()
@@ -366,7 +367,8 @@ class Engine:
     def commit_tree(self, tree: TreeStep, picks: torch.Tensor) -> List[List[int]]:
         """Takes over what the picks (int32 [nodes] on the device, in the order of the logits' rows: the token chosen after each
         node) agree with: from a tree's first node on, the child whose token is the pick, as long as there is one.  The slots then
-        hold the accepted tokens.  Returns, for every entry, the accepted nodes' tokens after the first, and behind them the pick after the last one."""
+        hold the accepted tokens, and no pages but those they lie in.  Returns, for every entry, the accepted nodes' tokens after the first, and
+        behind them the pick after the last one."""
         from ..kernels import ops
         if tree.done:
             raise RuntimeError("this step has been committed already")
@@ -384,6 +386,7 @@ class Engine:
         accepted = []
         for e, nodes, n, last in zip(tree.entries, path, counts, nexts):
             self.cache.commit(e.slot, self.cache.length(e.slot) + n)
+            self.cache.truncate(e.slot, self.cache.length(e.slot))       # pages that only nodes left behind lie in are for others to take
             accepted.append([int(e.tokens[i]) for i in nodes[1:n]] + [last])
         return accepted
 

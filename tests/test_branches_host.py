@@ -174,6 +174,28 @@ def test_pages_beyond_a_shared_length_are_not_shared_when_written():
     m.check()
 
 
+def test_rewinding_to_the_own_length_gives_spare_pages_back():
+    """What was reserved and not kept goes back, to the pool or to its other holders, and the slot goes on as before."""
+    for window, state in ((None, False), (None, True), (100, False)):
+        c = make_cache(window=window, state=state)
+        m = Mirror(c)
+        a = m.open()
+        m.write([a], 130)
+        m.check()
+        free = c.free_pages
+        c.reserve([(a, 130 + 200)])
+        assert c.free_pages < free
+        b = c.fork(a)
+        m.rows[b], m.states[b] = list(m.rows[a]), m.states[a]
+        for s in (a, b):
+            assert c.truncate(s, 130) == 130 == c.length(s)
+        assert c.free_pages == free
+        m.check()
+        m.write([a, b], 70)
+        m.check()
+        assert c.truncate(a, 10 ** 6) == 200
+
+
 def test_reordering_refuses_what_is_no_permutation_of_open_slots():
     c = make_cache()
     a, b = c.open_slot(), c.open_slot()

@@ -169,6 +169,36 @@ def test_drafted_generation_at_the_ends_of_context_and_pool(model_dirs, tiny_con
         assert [r.finish_reason for r in llm.generate_drafted(prompts, max_new=0)] == ["length"] * 2
 
 
+def test_rejected_drafts_keep_no_pages(model_dirs, tiny_configs):
+    """A pool that just holds what one-token steps need is enough however many drafts are rejected."""
+    d = model_dirs("D", "float32")
+    llm = gi.LLM(d, dtype="float32", max_tokens=64 * 3)
+    vocab = llm.engine.vocab
+    prompts = [tokens_for(tiny_configs["D"], n, n) for n in (34, 60)]
+    want = llm.generate(prompts, max_new=60, temperature=0.0, batch_size=2, stop_token_ids=())
+    assert [r.finish_reason for r in want] == ["capacity"] * 2 and len(want[1].tokens) > 20      # (the second went on into the third page)
+    run = prompts[0] + want[0].tokens
+
+    def wrong(tokens, most):
+        if tokens[:34] != prompts[0] or len(tokens) >= len(run):
+            return [], []
+        return [(run[len(tokens)] + 1) % vocab] * most, [-1] + list(range(most - 1))
+
+    got = llm.generate_drafted(prompts, max_new=60, drafter=wrong, batch_size=2, stop_token_ids=())
+    assert [(r.tokens, r.finish_reason) for r in got] == [(r.tokens, r.finish_reason) for r in want]
+    # and step by step: a slot holds the pages of its accepted tokens, an uncommitted step's go back on demand
+    eng = llm.engine
+    s = eng.cache.open_slot()
+    eng.step([StepEntry(s, prompts[0])])
+    step = eng.step_tree([TreeEntry(s, [1] * 100, [-1] + list(range(99)))])
+    assert eng.cache.free_pages == 0
+    eng.commit_tree(step, torch.full((100,), 2, dtype=torch.int32, device="cuda:0"))
+    assert eng.cache.length(s) == 35 and eng.cache.free_pages == 2
+    eng.step_tree([TreeEntry(s, [1] * 100, [-1] + list(range(99)))])
+    assert eng.cache.free_pages == 0 and eng.cache.truncate(s, 35) == 35 and eng.cache.free_pages == 2
+    eng.cache.close_slot(s)
+
+
 def test_drafted_generation_says_how_long_it_took(model_dirs, tiny_configs):
     llm = gi.LLM(model_dirs("A", "float32"), dtype="float32", max_tokens=64 * 40)
     prompts = [tokens_for(tiny_configs["A"], n, n) for n in (20, 3)]
