@@ -14,6 +14,8 @@
 // Bound: 32-bit multiply-adds (2 per query number and key) with many rows, the cache's bytes with few.  B200, 3 trees of 5 to 17
 // nodes behind 100 to 701 positions, 32 heads of 64 over 8: 20 us with the join (two tiles a block 30; breaks inside the inner loops
 // for rows that are not there 33; the body for 16 rows beside the one for 64 chosen by unit instead).
+#include <float.h>
+
 #include <type_traits>
 
 #include "api.h"
@@ -442,8 +444,9 @@ extern "C" int gi_attn_tree(void* out, long ldo, const void* q, long ldq, long q
   if (words < (max_nodes + 31) / 32) return gi::fail(GI_ERR_ARG, "tree attention: %d words of mask bits cannot hold %d nodes", words, max_nodes);
   if (n_seqs > MAX_SEQS) return gi::fail(GI_ERR_UNSUPPORTED, "tree attention: more than %d sequences in one launch", MAX_SEQS);
   if (cache_pages < 1 || max_pages < 1 || max_kv_len < 1) return gi::fail(GI_ERR_ARG, "tree attention: %d pages, %d in a table's row, %d positions", cache_pages, max_pages, max_kv_len);
-  // tensor cores: 16-bit rows and pages that TMA and 16-byte accesses can take, row coordinates of 32 bits
-  const bool tensor = dtype == GI_BF16 && (hd == 64 || hd == 128) && n_heads / n_kv <= 128 && q_rows <= 0x7fffffffL && ldq % 8 == 0 && ldo % 8 == 0 && (((uintptr_t)q | (uintptr_t)kcache | (uintptr_t)vcache | (uintptr_t)out) & 15) == 0 &&
+  // tensor cores: 16-bit rows and pages that TMA and 16-byte accesses can take, row coordinates of 32 bits; a scale above zero (that form
+  // hides scores before it scales them: -inf times nothing is no number, times less than nothing the largest of all)
+  const bool tensor = dtype == GI_BF16 && (hd == 64 || hd == 128) && scale >= FLT_MIN && scale <= FLT_MAX && n_heads / n_kv <= 128 && q_rows <= 0x7fffffffL && ldq % 8 == 0 && ldo % 8 == 0 && (((uintptr_t)q | (uintptr_t)kcache | (uintptr_t)vcache | (uintptr_t)out) & 15) == 0 &&
                       (long)cache_pages * n_kv * PAGE_TOKENS <= 0x7fffffffL;
   const Plan p = plan_of(n_seqs, max_nodes, max_kv_len, n_heads, n_kv, tensor);
   if (scratch_bytes < gi_attn_tree_scratch(n_seqs, max_nodes, max_kv_len, n_heads, n_kv, hd, dtype) || ((uintptr_t)scratch & 15))

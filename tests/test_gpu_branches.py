@@ -500,6 +500,21 @@ def test_tree_attention_one_long_context_over_all_blocks(dtype, dim):
     c.check(c.run())
 
 
+@pytest.mark.parametrize("dtype,dim", [(F32, 64), (BF16, 64), (BF16, 128), (BF16, 80)])
+@pytest.mark.parametrize("scale", ["none", "tiny", "negative"])
+def test_tree_attention_scales_of_any_sign(dtype, dim, scale):
+    """What a node does not see stays unseen whatever scores are multiplied with."""
+    rng = np.random.default_rng(3)
+    sizes, pos0 = [30, 20], [100, 0]
+    seen = [rng.random((n, n)) < 0.4 for n in sizes]
+    seen[1][5] = False
+    c = TreeCase(sizes, pos0, 4, 2, dim, dtype, seed=4, seen=seen)
+    got = c.run(scale={"none": 0.0, "tiny": 1e-40, "negative": -dim ** -0.5}[scale])
+    c.q = -c.q if scale == "negative" else torch.zeros_like(c.q)          # the same scores from a positive scale
+    c.check(got)
+    assert (got[35] == 0).all()
+
+
 def test_tree_attention_graph_and_streams():
     """A recorded launch serves other lengths, trees and tokens; calls on two streams do not meet."""
     for dtype in (F32, BF16):
