@@ -374,10 +374,21 @@ struct Plan {
   bool many_parts;      // a unit lies on more than a few blocks
 };
 
+// Shared memory of a block of the form on CUDA cores: queries, a tile's keys and values, weights.
+constexpr size_t smem_of(int rows_block, int hd) { return ((size_t)(rows_block + 2 * TILE) * ((hd + 3) / 4 * 4 + 4) + (size_t)rows_block * 68) * sizeof(float); }
+
+// Blocks of it that an SM holds: two with their registers (__launch_bounds__), one where two blocks' shared memory, the lengths' list
+// and 1 KB of the system's among it, is more than 228 KB (64 rows of heads above 116 numbers, 16 rows of heads above 180).  Ranges for
+// two where one fits come in two waves, with twice the parts to join: 32 32-bit heads of 128 over 8 behind 1,500 positions, one tree of
+// 26 nodes 57 us for 43, 8 trees of 16 nodes 163 for 149, of 64 nodes 533 for 540.
+int blocks_of_sm(int rows_block, int hd) {
+  return 2 * (smem_of(rows_block, hd) + 4 * (MAX_SEQS + 1) + 1024) <= 228 * 1024 && !(rows_block == 64 && hd > 128) ? 2 : 1;
+}
+
 // The query rows of a block: 16 or 64 on CUDA cores, the smaller where it takes a tree's rows; on tensor cores as many whole nodes as
 // 128 lanes hold, and up to 8 row blocks of a unit side by side.  Blocks: as many as the device runs at a time, fewer if
 // there are not `least` tiles for each.
-Plan plan_of(int n_seqs, int max_nodes, int max_kv_len, int n_heads, int n_kv, bool tensor) {
+Plan plan_of(int n_seqs, int max_nodes, int max_kv_len, int n_heads, int n_kv, int hd, bool tensor) {
   Plan p;
   const int group = n_heads / n_kv;
   const long rows = (long)max_nodes * group;
@@ -388,7 +399,7 @@ Plan plan_of(int n_seqs, int max_nodes, int max_kv_len, int n_heads, int n_kv, b
   p.split = (int)((blocks + rounds - 1) / rounds);
   const long units = (long)n_seqs * n_kv * rounds, tiles = (max_kv_len + p.tile - 1) / p.tile;
   const long wanted = units * ((tiles + p.least - 1) / p.least);
-  const long cap = (tensor ? 1L : 2L) * gi::sm_count() / p.split;
+  const long cap = (tensor ? 1L : (long)blocks_of_sm(p.rows_block, hd)) * gi::sm_count() / p.split;
   p.ranges = (int)(wanted < cap ? wanted : cap);
   if (p.ranges < 1) p.ranges = 1;
   p.many_parts = p.ranges > 3 * units;
@@ -400,14 +411,12 @@ long scratch_of(const Plan& p, int n_seqs, int hd) { return 4L * ((n_seqs + 4) /
 template <typename T, int R, int DCH>
 int launch_tree(const Shape& sh, const Plan& p, T* out, long ldo, const T* q, long ldq, const T* k, const T* v, int hd, float scale,
                 float4* part_o, float2* part_ml, int* part_prefix, cudaStream_t s) {
-  const int hp = (hd + 3) / 4 * 4;
-  const size_t smem = ((size_t)(R + 2 * TILE) * (hp + 4) + (size_t)R * 68) * sizeof(float);
+  const size_t smem = smem_of(R, hd);
   auto kern = attn_tree_kernel<T, R, DCH>;
   static bool configured[gi::MAX_DEVICES_SEEN] = {false};
   int dev;
   if (gi::unconfigured_here(configured, &dev)) {
-    const size_t most = ((size_t)(R + 2 * TILE) * (DCH * 64 + 4) + (size_t)R * 68) * sizeof(float);
-    cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)most);
+    cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem_of(R, DCH * 64));
     if (e != cudaSuccess) return gi::fail(GI_ERR_CUDA, "tree attention: %s", cudaGetErrorString(e));
     if (dev >= 0) configured[dev] = true;
   }
@@ -427,9 +436,9 @@ int launch_tree_dims(const Shape& sh, const Plan& p, T* out, long ldo, const T* 
 
 extern "C" long gi_attn_tree_scratch(int n_seqs, int max_nodes, int max_kv_len, int n_heads, int n_kv, int hd, int dtype) {
   if (n_seqs <= 0 || max_nodes <= 0 || max_kv_len <= 0 || n_kv <= 0 || n_heads < n_kv || hd <= 0) return 0;
-  const long plain = scratch_of(plan_of(n_seqs, max_nodes, max_kv_len, n_heads, n_kv, false), n_seqs, hd);
+  const long plain = scratch_of(plan_of(n_seqs, max_nodes, max_kv_len, n_heads, n_kv, hd, false), n_seqs, hd);
   if (dtype != GI_BF16 || (hd != 64 && hd != 128) || n_heads / n_kv > 128) return plain;
-  const long tensor = scratch_of(plan_of(n_seqs, max_nodes, max_kv_len, n_heads, n_kv, true), n_seqs, hd);
+  const long tensor = scratch_of(plan_of(n_seqs, max_nodes, max_kv_len, n_heads, n_kv, hd, true), n_seqs, hd);
   return tensor > plain ? tensor : plain;
 }
 
@@ -448,7 +457,7 @@ extern "C" int gi_attn_tree(void* out, long ldo, const void* q, long ldq, long q
   // hides scores before it scales them: -inf times nothing is no number, times less than nothing the largest of all)
   const bool tensor = dtype == GI_BF16 && (hd == 64 || hd == 128) && scale >= FLT_MIN && scale <= FLT_MAX && n_heads / n_kv <= 128 && q_rows <= 0x7fffffffL && ldq % 8 == 0 && ldo % 8 == 0 && (((uintptr_t)q | (uintptr_t)kcache | (uintptr_t)vcache | (uintptr_t)out) & 15) == 0 &&
                       (long)cache_pages * n_kv * PAGE_TOKENS <= 0x7fffffffL;
-  const Plan p = plan_of(n_seqs, max_nodes, max_kv_len, n_heads, n_kv, tensor);
+  const Plan p = plan_of(n_seqs, max_nodes, max_kv_len, n_heads, n_kv, hd, tensor);
   if (scratch_bytes < gi_attn_tree_scratch(n_seqs, max_nodes, max_kv_len, n_heads, n_kv, hd, dtype) || ((uintptr_t)scratch & 15))
     return gi::fail(GI_ERR_ARG, "tree attention: the scratch memory is too small or not aligned");
   // the list of tiles is counted in 32 bits

@@ -515,6 +515,15 @@ def test_tree_attention_scales_of_any_sign(dtype, dim, scale):
     assert (got[35] == 0).all()
 
 
+@pytest.mark.parametrize("nodes,dim,a_sm", [(16, 64, 2), (16, 112, 2), (16, 128, 1), (16, 256, 1), (4, 128, 2), (4, 180, 2), (4, 184, 1), (4, 256, 1)])
+def test_tree_attention_has_as_many_blocks_as_the_sms_hold(nodes, dim, a_sm):
+    """A job that fills the device: the scratch memory holds two partial results of 64 or 16 rows for every block that fits at a time."""
+    nbytes = ops._bind().gi_attn_tree_scratch(64, nodes, 100000, 32, 8, dim, 0)
+    rows = 64 if nodes == 16 else 16
+    sms = torch.cuda.get_device_properties(0).multi_processor_count
+    assert nbytes == 4 * 68 + 2 * a_sm * sms * rows * (dim + 2) * 4
+
+
 def test_tree_attention_graph_and_streams():
     """A recorded launch serves other lengths, trees and tokens; calls on two streams do not meet."""
     for dtype in (F32, BF16):
