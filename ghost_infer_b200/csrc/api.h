@@ -696,12 +696,14 @@ int gi_copy_pages(const long* tensors, int n, const int* src, const int* dst, co
 // before seq_pos0[b] and the nodes in its row of `masks` ([tokens][words] 32-bit words, bit i of word w: node 32 w + i).  A node
 // that sees nothing gets zeros.  max_kv_len (cached positions and nodes of the longest sequence) and max_nodes size the launch; a
 // max_kv_len that is too small costs time only.  hd 1 to 256, n_seqs at most 1024.  scratch: gi_attn_tree_scratch bytes, 16-byte
-// aligned.  Keys and values of nodes that nobody sees, and what lies behind the last node, may hold anything.
+// aligned.  Keys and values of nodes that nobody sees, and what lies behind the last node, may hold anything.  Nothing outside the q_rows
+// rows, the table's rows and the cache's pages is read or written, whatever lengths, slots and tables say: a slot that the table does not
+// have reads the trash page.
 long gi_attn_tree_scratch(int n_seqs, int max_nodes, int max_kv_len, int n_heads, int n_kv, int hd, int dtype);
 int gi_attn_tree(void* out, long ldo, const void* q, long ldq, long q_rows, int dtype, const void* kcache, const void* vcache, int cache_pages,
-                 const int* block_table, int max_pages, const int* cu_seqlens, const int* seq_slots, const int* seq_pos0, const int* masks,
-                 int words, int n_seqs, int max_nodes, int max_kv_len, int n_heads, int n_kv, int hd, float scale, void* scratch,
-                 long scratch_bytes, void* stream);
+                 const int* block_table, int table_rows, int max_pages, const int* cu_seqlens, const int* seq_slots, const int* seq_pos0,
+                 const int* masks, int words, int n_seqs, int max_nodes, int max_kv_len, int n_heads, int n_kv, int hd, float scale,
+                 void* scratch, long scratch_bytes, void* stream);
 // Nonzero: a bounded wait of the tensor-core form ran out since the last question (and asks for it once).
 int gi_attn_tree_status(int* status);
 
@@ -709,10 +711,11 @@ int gi_attn_tree_status(int* status);
 // is this node) whose token is the node's pick, as long as there is one.  out_path [n_seqs][max_nodes]: the accepted nodes, then -1;
 // out_counts; out_next: the last accepted node's pick (-1 for no nodes).  The accepted nodes' rows move from position
 // seq_pos0 + node to seq_pos0 + place in the path, in every layer and head of `n` (0 to 8) tensors of pages (as gi_copy_pages).
-// A slot of -1 moves nothing; positions outside the table or pages outside a tensor are passed over.  max_nodes 1 to 256.
+// A slot of -1, or one that the table does not have, moves nothing; positions outside the table, pages outside a tensor and nodes past the
+// n_tokens tokens are passed over.  max_nodes 1 to 256.
 int gi_tree_commit(int* out_path, int* out_counts, int* out_next, const int* picks, const int* tokens, const int* parents,
-                   const int* cu_seqlens, const int* seq_slots, const int* seq_pos0, int n_seqs, int max_nodes, const long* tensors,
-                   int n, const int* block_table, int max_pages, void* stream);
+                   int n_tokens, const int* cu_seqlens, const int* seq_slots, const int* seq_pos0, int n_seqs, int max_nodes,
+                   const long* tensors, int n, const int* block_table, int table_rows, int max_pages, void* stream);
 
 #ifdef __cplusplus
 }

@@ -443,7 +443,7 @@ extern "C" long gi_attn_tree_scratch(int n_seqs, int max_nodes, int max_kv_len, 
 }
 
 extern "C" int gi_attn_tree(void* out, long ldo, const void* q, long ldq, long q_rows, int dtype, const void* kcache, const void* vcache, int cache_pages,
-                            const int* block_table, int max_pages, const int* cu_seqlens, const int* seq_slots, const int* seq_pos0, const int* masks,
+                            const int* block_table, int table_rows, int max_pages, const int* cu_seqlens, const int* seq_slots, const int* seq_pos0, const int* masks,
                             int words, int n_seqs, int max_nodes, int max_kv_len, int n_heads, int n_kv, int hd, float scale, void* scratch,
                             long scratch_bytes, void* stream) {
   if (n_seqs <= 0 || q_rows <= 0) return GI_OK;
@@ -452,7 +452,7 @@ extern "C" int gi_attn_tree(void* out, long ldo, const void* q, long ldq, long q
   if (max_nodes < 1 || max_nodes > MAX_NODES) return gi::fail(GI_ERR_ARG, "tree attention: trees of up to %d nodes, 1 to %d are supported", max_nodes, MAX_NODES);
   if (words < (max_nodes + 31) / 32) return gi::fail(GI_ERR_ARG, "tree attention: %d words of mask bits cannot hold %d nodes", words, max_nodes);
   if (n_seqs > MAX_SEQS) return gi::fail(GI_ERR_UNSUPPORTED, "tree attention: more than %d sequences in one launch", MAX_SEQS);
-  if (cache_pages < 1 || max_pages < 1 || max_kv_len < 1) return gi::fail(GI_ERR_ARG, "tree attention: %d pages, %d in a table's row, %d positions", cache_pages, max_pages, max_kv_len);
+  if (cache_pages < 1 || table_rows < 0 || max_pages < 1 || max_kv_len < 1) return gi::fail(GI_ERR_ARG, "tree attention: %d pages, %d in a table's row, %d positions", cache_pages, max_pages, max_kv_len);
   // tensor cores: 16-bit rows and pages that TMA and 16-byte accesses can take, row coordinates of 32 bits; a scale above zero (that form
   // hides scores before it scales them: -inf times nothing is no number, times less than nothing the largest of all)
   const bool tensor = dtype == GI_BF16 && (hd == 64 || hd == 128) && scale >= FLT_MIN && scale <= FLT_MAX && n_heads / n_kv <= 128 && q_rows <= 0x7fffffffL && ldq % 8 == 0 && ldo % 8 == 0 && (((uintptr_t)q | (uintptr_t)kcache | (uintptr_t)vcache | (uintptr_t)out) & 15) == 0 &&
@@ -463,7 +463,7 @@ extern "C" int gi_attn_tree(void* out, long ldo, const void* q, long ldq, long q
   // the list of tiles is counted in 32 bits
   const long most = (long)n_seqs * n_kv * (((long)max_nodes * (n_heads / n_kv) + p.rows_block - 1) / p.rows_block) * (((long)max_pages * PAGE_TOKENS + max_nodes) / p.tile + 1);
   if (most > 0x3fffffffL || max_pages > 0x7fffffff / PAGE_TOKENS - MAX_NODES) return gi::fail(GI_ERR_UNSUPPORTED, "tree attention: %d sequences of up to %d pages are more than one launch takes", n_seqs, max_pages);
-  const Shape sh = {cu_seqlens, seq_slots, seq_pos0, block_table, masks, words, max_pages, n_seqs, n_heads, n_kv, max_nodes, cache_pages, p.rows_block, p.split, p.tile, p.least};
+  const Shape sh = {cu_seqlens, seq_slots, seq_pos0, block_table, masks, words, table_rows, max_pages, n_seqs, n_heads, n_kv, max_nodes, cache_pages, q_rows, p.rows_block, p.split, p.tile, p.least};
   int* prefix_out = (int*)scratch;
   float4* part_o = (float4*)(prefix_out + (n_seqs + 4) / 4 * 4);
   float2* part_ml = (float2*)(part_o + 2L * p.ranges * p.split * p.rows_block * ((hd + 3) / 4));

@@ -27,7 +27,8 @@ struct Shape {
   const int* seq_pos0;
   const int* block_table;
   const int* masks;       // [tokens][words] bits: the nodes of its own tree that a token sees
-  int words, max_pages, n_seqs, n_heads, n_kv, max_nodes, cache_pages;
+  int words, table_rows, max_pages, n_seqs, n_heads, n_kv, max_nodes, cache_pages;
+  long tokens;            // rows of queries, masks and output
   int rows_block;         // query rows of a row block
   int split;              // row blocks of a unit, one to each of so many neighbouring blocks
   int tile;               // positions of a tile: 64 or 128
@@ -40,7 +41,11 @@ struct Unit {
   int tiles, first;       // tiles, the first one's place in the launch's list
 };
 
-__device__ __forceinline__ int nodes_of(const Shape& s, int b) { return max(0, min(s.cu_seqlens[b + 1] - s.cu_seqlens[b], s.max_nodes)); }
+// (offsets that the rows do not hold name no node)
+__device__ __forceinline__ int nodes_of(const Shape& s, int b) {
+  const int first = s.cu_seqlens[b], end = (int)min((long)s.cu_seqlens[b + 1], s.tokens);
+  return first < 0 ? 0 : max(0, min(end - first, s.max_nodes));
+}
 
 // (a length that the page table cannot hold is cut off: the entry point bounds the list by the table's)
 __device__ __forceinline__ int pos0_of(const Shape& s, int b) { return max(0, min(s.seq_pos0[b], s.max_pages * PAGE_TOKENS)); }
@@ -112,9 +117,9 @@ __device__ __forceinline__ size_t part_at(const Shape& s, size_t slot, int fours
 }
 
 // The cache's page that holds a sequence's positions from 64 * index on.  A table may hold anything behind a sequence's end and in
-// an unused slot: what is no page of the cache reads as the trash page.
+// an unused slot: what is no page of the cache, and a slot that the table does not have, reads as the trash page.
 __device__ __forceinline__ int page_of(const Shape& s, int slot, int index) {
-  if (slot < 0 || index >= s.max_pages) return 0;
+  if (slot < 0 || slot >= s.table_rows || index >= s.max_pages) return 0;
   const int page = s.block_table[(size_t)slot * s.max_pages + index];
   return page >= 0 && page < s.cache_pages ? page : 0;
 }

@@ -22,14 +22,14 @@ constexpr int MAX_NODES = 256;
 template <typename V>
 __global__ void __launch_bounds__(THREADS)
 tree_commit_kernel(const __grid_constant__ gi::PageTensors t, int n_tensors, const int* picks, const int* tokens, const int* parents,
-                   const int* cu_seqlens, const int* seq_slots, const int* seq_pos0, const int* block_table, int max_pages, int max_nodes,
+                   int n_tokens, const int* cu_seqlens, const int* seq_slots, const int* seq_pos0, const int* block_table, int table_rows, int max_pages, int max_nodes,
                    int* __restrict__ out_path, int* __restrict__ out_counts, int* __restrict__ out_next) {
   __shared__ int s_token[MAX_NODES], s_parent[MAX_NODES], s_pick[MAX_NODES], s_path[MAX_NODES], s_page[MAX_NODES / PAGE_TOKENS + 2];
   __shared__ int s_count;
   const int tid = threadIdx.x, lane = tid & 31, b = blockIdx.y;
   gi::pdl_prologue();
-  const int tok0 = cu_seqlens[b], n = min(cu_seqlens[b + 1] - tok0, max_nodes);
-  const int slot = seq_slots[b], pos0 = seq_pos0[b];
+  const int tok0 = cu_seqlens[b], end = min(cu_seqlens[b + 1], n_tokens), slot = seq_slots[b], pos0 = seq_pos0[b];
+  const int n = tok0 < 0 ? 0 : min(end - tok0, max_nodes);
   for (int i = tid; i < n; i += THREADS) {
     s_token[i] = tokens[tok0 + i];
     s_parent[i] = parents[tok0 + i];
@@ -37,7 +37,7 @@ tree_commit_kernel(const __grid_constant__ gi::PageTensors t, int n_tensors, con
   }
   const int page0 = pos0 / PAGE_TOKENS, n_pages = MAX_NODES / PAGE_TOKENS + 2;
   for (int i = tid; i < n_pages; i += THREADS)
-    s_page[i] = slot >= 0 && pos0 >= 0 && page0 + i < max_pages ? block_table[(size_t)slot * max_pages + page0 + i] : -1;
+    s_page[i] = slot >= 0 && slot < table_rows && pos0 >= 0 && page0 + i < max_pages ? block_table[(size_t)slot * max_pages + page0 + i] : -1;
   __syncthreads();
   if (tid < 32) {
     int count = 0, at = 0;
@@ -109,8 +109,8 @@ tree_commit_kernel(const __grid_constant__ gi::PageTensors t, int n_tensors, con
 }  // namespace
 
 extern "C" int gi_tree_commit(int* out_path, int* out_counts, int* out_next, const int* picks, const int* tokens, const int* parents,
-                              const int* cu_seqlens, const int* seq_slots, const int* seq_pos0, int n_seqs, int max_nodes, const long* tensors,
-                              int n, const int* block_table, int max_pages, void* stream) {
+                              int n_tokens, const int* cu_seqlens, const int* seq_slots, const int* seq_pos0, int n_seqs, int max_nodes,
+                              const long* tensors, int n, const int* block_table, int table_rows, int max_pages, void* stream) {
   if (n_seqs <= 0) return GI_OK;
   if (max_nodes < 1 || max_nodes > MAX_NODES) return gi::fail(GI_ERR_ARG, "tree commit: trees of up to %d nodes, 1 to %d are supported", max_nodes, MAX_NODES);
   if (n_seqs > 65535) return gi::fail(GI_ERR_UNSUPPORTED, "tree commit: more than 65535 sequences in one launch");
@@ -124,8 +124,8 @@ extern "C" int gi_tree_commit(int* out_path, int* out_counts, int* out_next, con
   if (blocks > 0x7fffffffL) return gi::fail(GI_ERR_UNSUPPORTED, "tree commit: more rows' columns than one launch holds");
   const dim3 grid((unsigned)blocks, n_seqs);
   cudaStream_t s = (cudaStream_t)stream;
-#define GI_TREE(V) gi::check(gi::launch(tree_commit_kernel<V>, grid, dim3(THREADS), 0, s, t, n, picks, tokens, parents, cu_seqlens, seq_slots, seq_pos0, \
-                                        block_table, max_pages, max_nodes, out_path, out_counts, out_next), "tree commit")
+#define GI_TREE(V) gi::check(gi::launch(tree_commit_kernel<V>, grid, dim3(THREADS), 0, s, t, n, picks, tokens, parents, n_tokens, cu_seqlens, seq_slots, seq_pos0, \
+                                        block_table, table_rows, max_pages, max_nodes, out_path, out_counts, out_next), "tree commit")
   if (unit == 16) return GI_TREE(uint4);
   if (unit == 4) return GI_TREE(unsigned);
   return GI_TREE(unsigned short);

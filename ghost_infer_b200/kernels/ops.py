@@ -159,10 +159,10 @@ def _bind():
         "gi_beam_select_scratch": [I, I, I],
         "gi_reorder_states": [P, I, I, P, P, I, I, I, P],
         "gi_copy_pages": [P, I, P, P, P, I, P],
-        "gi_attn_tree": [P, L, P, L, L, I, P, P, I, P, I, P, P, P, P, I, I, I, I, I, I, I, F, P, L, P],
+        "gi_attn_tree": [P, L, P, L, L, I, P, P, I, P, I, I, P, P, P, P, I, I, I, I, I, I, I, F, P, L, P],
         "gi_attn_tree_scratch": [I, I, I, I, I, I, I],
         "gi_attn_tree_status": [P],
-        "gi_tree_commit": [P, P, P, P, P, P, P, P, P, I, I, P, I, P, I, P],
+        "gi_tree_commit": [P, P, P, P, P, P, I, P, P, P, I, I, P, I, P, I, I, P],
         "gi_attn_decode_generic_ex3": [P, L, P, P, P, L, I, P, P, P, I, P, P, I, I, I, I, F, I, I, I, I, F, P, I, L, I, P],
     }
     for name, argtypes in sigs.items():
@@ -3022,7 +3022,8 @@ def attention_tree(q: torch.Tensor, kcache: torch.Tensor, vcache: torch.Tensor, 
     (`cu_seqlens`, at most `max_nodes` <= 256) are the nodes of a tree, cached at the positions seq_pos0[b] + node; a node sees
     all positions before seq_pos0[b] and the nodes that its row of `masks` names (int32 [tokens, words], bit i of word w: node
     32 w + i).  A node that sees nothing gets zeros.  `q`: rows whose first n_heads * head_dim columns are the queries.
-    `max_kv_len`: positions and nodes of the longest sequence (sizes the launch; too small a number costs time only)."""
+    `max_kv_len`: positions and nodes of the longest sequence (sizes the launch; too small a number costs time only).  A slot that
+    `block_table` does not have reads the trash page; nodes past the rows of `q` are left out."""
     lib = _bind()
     stream = _on_here("tree attention", q, kcache, vcache, block_table, cu_seqlens, seq_slots, seq_pos0, masks, out)
     _cuda(q, "queries")
@@ -3042,7 +3043,7 @@ def attention_tree(q: torch.Tensor, kcache: torch.Tensor, vcache: torch.Tensor, 
     nbytes = lib.gi_attn_tree_scratch(n_seqs, max_nodes, max_kv_len, n_heads, n_kv, head_dim, dt)
     scratch = masks.new_empty((nbytes // 4,))
     _check(lib, lib.gi_attn_tree(out.data_ptr(), ldo, q.data_ptr(), ldq, rows, dt, kcache.data_ptr(), vcache.data_ptr(), kcache.shape[0],
-                                 _i32_rows(block_table, "block table"), block_table.shape[1], cu, ss, sp, mp, masks.shape[1], n_seqs, max_nodes,
+                                 _i32_rows(block_table, "block table"), *block_table.shape, cu, ss, sp, mp, masks.shape[1], n_seqs, max_nodes,
                                  max_kv_len, n_heads, n_kv, head_dim, scale, scratch.data_ptr(), nbytes, stream), 2 if n_seqs else 0)
     return out
 
@@ -3054,7 +3055,7 @@ def tree_commit(picks: torch.Tensor, tokens: torch.Tensor, parents: torch.Tensor
     picks, tokens, parents: int32 [tokens].  Returns path int32 [sequences, max_nodes] (accepted nodes, then -1), counts and
     next tokens (the last accepted node's pick; -1 without nodes), int32 [sequences].  In the storage tensors `pages`
     ([layers, pages, heads, 64, numbers], at most 8, or none) the accepted rows move from position seq_pos0 + node to
-    seq_pos0 + place in the path; a slot of -1 moves nothing."""
+    seq_pos0 + place in the path; a slot that `block_table` does not have (-1, say) moves nothing, nodes past the tokens are left out."""
     lib = _bind()
     pages = list(pages)
     stream = _on_here("tree commit", picks, tokens, parents, cu_seqlens, seq_slots, seq_pos0, block_table, *pages)
@@ -3066,7 +3067,7 @@ def tree_commit(picks: torch.Tensor, tokens: torch.Tensor, parents: torch.Tensor
     path = picks.new_empty((n_seqs, max_nodes))
     counts = picks.new_empty((n_seqs,))
     nexts = torch.empty_like(counts)
-    _check(lib, lib.gi_tree_commit(path.data_ptr(), counts.data_ptr(), nexts.data_ptr(), pk, tk, pr, cu, ss, sp, n_seqs, max_nodes,
-                                   _page_tensors(pages, "tree commit"), len(pages), _i32_rows(block_table, "block table"), block_table.shape[1], stream),
+    _check(lib, lib.gi_tree_commit(path.data_ptr(), counts.data_ptr(), nexts.data_ptr(), pk, tk, pr, total, cu, ss, sp, n_seqs, max_nodes,
+                                   _page_tensors(pages, "tree commit"), len(pages), _i32_rows(block_table, "block table"), *block_table.shape, stream),
            1 if n_seqs else 0)
     return path, counts, nexts

@@ -464,6 +464,37 @@ def test_tree_attention_rows_on_any_boundary(dtype, dim, shift):
     c.check(want)
 
 
+@pytest.mark.parametrize("dtype,dim", [(F32, 64), (BF16, 128), (BF16, 72)])
+def test_tree_attention_slots_and_lengths_that_are_not_there(dtype, dim):
+    """A slot past the table's last row reads the trash page, as -1 does; offsets past the rows leave the rest out."""
+    c = TreeCase([9, 30], [130, 77], 4, 2, dim, dtype, seed=8)
+    want = c.run()
+    c.k[0], c.v[0] = 0.5, 0.25
+    for slot in (2, 1 << 20, -1, -(1 << 30)):
+        got = c.run(seq_slots=i32([c.slots[0], slot]))
+        # (107 keys at most: the sums of weights and of values, a weight's and the result's rounding to 16 bits)
+        off = 0.25 * (2 * 107 * 2.0 ** -24 + (2.0 ** -7 + 2.0 ** -15 if dtype == BF16 else 2.0 ** -23))
+        assert torch.equal(got[:9], want[:9]) and ((got[9:].float() - 0.25).abs() <= off).all()
+    wide = torch.full((60, 4 * dim), 3.0, dtype=dtype, device=DEV)
+    got = c.run(cu_seqlens=i32([0, 9, 50]), max_nodes=50, out=wide[:39], masks=torch.cat([c.masks, torch.zeros_like(c.masks)], dim=1))
+    assert torch.equal(got[:9], want[:9]) and (wide[39:] == 3).all()
+    c.check(c.run(cu_seqlens=i32([0, 9, 2000]), max_nodes=30, seq_pos0=c.pos0_dev))
+    for cu in ([-5, 0, 0], [50, 60, 70], [0, 0, -3]):
+        assert (c.run(cu_seqlens=i32(cu)) == 7).all()
+
+
+def test_tree_commit_slots_and_lengths_that_are_not_there():
+    pages = [randn(1, 3, 1, 64, 8, seed=1)]
+    want = pages[0].clone()
+    for slot in (1, 1 << 20):
+        path, counts, nexts = ops.tree_commit(i32([5, 5, 5]), i32([0, 4, 5]), i32([-1, 0, 0]), i32([0, 3]), i32([slot]), i32([0]), 1, 3, pages, i32([[1]]))
+        assert path.tolist() == [[0, 2, -1]] and torch.equal(pages[0], want)
+    for cu in ([0, 200], [-4, 3], [7, 9]):
+        path, counts, nexts = ops.tree_commit(i32([5, 5, 5]), i32([0, 4, 6]), i32([-1, 0, 0]), i32(cu), i32([0]), i32([0]), 1, 8, pages, i32([[1]]))
+        n = 1 if cu[0] == 0 else 0
+        assert counts.tolist() == [n] and path[0].tolist() == [0] * n + [-1] * (8 - n) and torch.equal(pages[0], want)
+
+
 def test_calls_with_nothing_to_do():
     none = i32([])
     out = torch.zeros((0, 64), dtype=BF16, device=DEV)
