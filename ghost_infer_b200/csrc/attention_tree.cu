@@ -43,7 +43,7 @@ attn_tree_kernel(const Shape sh, T* __restrict__ out, long ldo, const T* q, long
   gi::pdl_prologue();
   if (tid < 32) prefix(sh, s_pre);
   __syncthreads();
-  const int total = s_pre[sh.n_seqs], per = per_range(sh, total, gridDim.x);
+  const int total = s_pre[sh.n_seqs], per = per_range(total, gridDim.x);
   if (blockIdx.x == 0)
     for (int i = tid; i <= sh.n_seqs; i += THREADS) part_prefix[i] = s_pre[i];
   const int lo = (int)min((long)total, (long)blockIdx.x * per), hi = min(total, lo + per);
@@ -300,7 +300,7 @@ attn_tree_join_kernel(const Shape sh, T* __restrict__ out, long ldo, int hd, int
   const int kvh = blockIdx.y, row = blockIdx.x / cuts * 32 + lane;
   const int part_group = warp % PARTS, four0 = ((blockIdx.x % cuts) * CUTS + warp / PARTS) * FOURS;
   const int total = part_prefix[sh.n_seqs], before = part_prefix[b], n = nodes_of(sh, b), pos0 = pos0_of(sh, b), tok0 = sh.cu_seqlens[b];
-  const int per = per_range(sh, total, ranges);
+  const int per = per_range(total, ranges);
   const int tiles = tiles_of(sh, pos0, n), row_block = row / sh.rows_block, r = row - row_block * sh.rows_block;
   const int first = before + (row_block / sh.split * sh.n_kv + kvh) * tiles;
   int c0 = 0, c1 = 0;
@@ -370,7 +370,7 @@ attn_tree_join_kernel(const Shape sh, T* __restrict__ out, long ldo, int hd, int
 }
 
 struct Plan {
-  int ranges, split, rows_block, tile, least;
+  int ranges, split, rows_block, tile;
   bool many_parts;      // a unit lies on more than a few blocks
 };
 
@@ -387,18 +387,17 @@ int blocks_of_sm(int rows_block, int hd) {
 
 // The query rows of a block: 16 or 64 on CUDA cores, the smaller where it takes a tree's rows; on tensor cores as many whole nodes as
 // 128 lanes hold, and up to 8 row blocks of a unit side by side.  Blocks: as many as the device runs at a time, fewer if
-// there are not `least` tiles for each.
+// there is not a tile for each.
 Plan plan_of(int n_seqs, int max_nodes, int max_kv_len, int n_heads, int n_kv, int hd, bool tensor) {
   Plan p;
   const int group = n_heads / n_kv;
   const long rows = (long)max_nodes * group;
   p.rows_block = tensor ? 128 / group * group : (rows > 16 ? 64 : 16);
   p.tile = tensor ? 128 : TILE;
-  p.least = 1;
   const long blocks = (rows + p.rows_block - 1) / p.rows_block, rounds = tensor ? (blocks + 7) / 8 : blocks;
   p.split = (int)((blocks + rounds - 1) / rounds);
   const long units = (long)n_seqs * n_kv * rounds, tiles = (max_kv_len + p.tile - 1) / p.tile;
-  const long wanted = units * ((tiles + p.least - 1) / p.least);
+  const long wanted = units * tiles;
   const long cap = (tensor ? 1L : (long)blocks_of_sm(p.rows_block, hd)) * gi::sm_count() / p.split;
   p.ranges = (int)(wanted < cap ? wanted : cap);
   if (p.ranges < 1) p.ranges = 1;
@@ -463,7 +462,7 @@ extern "C" int gi_attn_tree(void* out, long ldo, const void* q, long ldq, long q
   // the list of tiles is counted in 32 bits
   const long most = (long)n_seqs * n_kv * (((long)max_nodes * (n_heads / n_kv) + p.rows_block - 1) / p.rows_block) * (((long)max_pages * PAGE_TOKENS + max_nodes) / p.tile + 1);
   if (most > 0x3fffffffL || max_pages > 0x7fffffff / PAGE_TOKENS - MAX_NODES) return gi::fail(GI_ERR_UNSUPPORTED, "tree attention: %d sequences of up to %d pages are more than one launch takes", n_seqs, max_pages);
-  const Shape sh = {cu_seqlens, seq_slots, seq_pos0, block_table, masks, words, table_rows, max_pages, n_seqs, n_heads, n_kv, max_nodes, cache_pages, q_rows, p.rows_block, p.split, p.tile, p.least};
+  const Shape sh = {cu_seqlens, seq_slots, seq_pos0, block_table, masks, words, table_rows, max_pages, n_seqs, n_heads, n_kv, max_nodes, cache_pages, q_rows, p.rows_block, p.split, p.tile};
   int* prefix_out = (int*)scratch;
   float4* part_o = (float4*)(prefix_out + (n_seqs + 4) / 4 * 4);
   float2* part_ml = (float2*)(part_o + 2L * p.ranges * p.split * p.rows_block * ((hd + 3) / 4));

@@ -32,7 +32,6 @@ struct Shape {
   int rows_block;         // query rows of a row block
   int split;              // row blocks of a unit, one to each of so many neighbouring blocks
   int tile;               // positions of a tile: 64 or 128
-  int least;              // tiles that a block's range has at least (unless the list ends)
 };
 
 struct Unit {
@@ -75,8 +74,8 @@ __device__ __forceinline__ void prefix(const Shape& s, int* out) {
   if (lane == 0) out[s.n_seqs] = upto;
 }
 
-// Tiles per range: equal ranges, but not so short that joining them would cost more than they save.
-__device__ __forceinline__ int per_range(const Shape& s, int total, int ranges) { return max((total + ranges - 1) / ranges, s.least); }
+// Tiles per range: equal ranges of one tile at least.
+__device__ __forceinline__ int per_range(int total, int ranges) { return max((total + ranges - 1) / ranges, 1); }
 
 // The unit that holds a tile of the list.
 __device__ __forceinline__ Unit unit_at(const Shape& s, const int* pre, int tile) {

@@ -159,7 +159,7 @@ attn_tree_t5_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
   tc_fence_after();
   const uint32_t tmem = *tmem_slot, tmem_o = tmem + 256;       // [score buffer][128 columns], then O [half of the keys][HD]
   const int ranges = gridDim.x / sh.split, range = blockIdx.x / sh.split, row_block = blockIdx.x % sh.split;
-  const int total = s_pre[sh.n_seqs], per = per_range(sh, total, ranges);
+  const int total = s_pre[sh.n_seqs], per = per_range(total, ranges);
   if (blockIdx.x == 0)
     for (int i = threadIdx.x; i <= sh.n_seqs; i += L::THREADS) part_prefix[i] = s_pre[i];
   const int lo = (int)min((long)total, (long)range * per), hi = min(total, lo + per);
