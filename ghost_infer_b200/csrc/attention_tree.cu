@@ -371,7 +371,7 @@ attn_tree_join_kernel(const Shape sh, T* __restrict__ out, long ldo, int hd, int
 
 struct Plan {
   int ranges, split, rows_block, tile;
-  bool many_parts;      // a unit lies on more than a few blocks
+  bool narrow_join;     // the join's blocks: 16 of a head's numbers and 8 warps to the parts, or 64 and 2
 };
 
 // Shared memory of a block of the form on CUDA cores: queries, a tile's keys and values, weights.
@@ -401,7 +401,11 @@ Plan plan_of(int n_seqs, int max_nodes, int max_kv_len, int n_heads, int n_kv, i
   const long cap = (tensor ? 1L : (long)blocks_of_sm(p.rows_block, hd)) * gi::sm_count() / p.split;
   p.ranges = (int)(wanted < cap ? wanted : cap);
   if (p.ranges < 1) p.ranges = 1;
-  p.many_parts = p.ranges > 3 * units;
+  // The narrow join has four times the blocks, each done sooner: right as long as the device holds them at a time, about 4 to an SM.  The
+  // whole call with the narrow / wide one, by the narrow one's blocks, 8 kv heads of groups of 4: bf16 heads of 128, 26 nodes, 256 blocks
+  // 15.8 / 21.4 us, 512 20.4 / 22.6, 768 27.6 / 27.5, 1,024 31.3 / 29.7; 90 nodes, 768 blocks 22.8 / 22.4, 1,536 35.9 / 31.2; heads of 64, 8
+  // nodes, 384 blocks 27.6 / 29.2, 512 32.5 / 32.2; 32-bit heads of 64, 12 nodes, 384 blocks 30.5 / 33.2, 448 41.4 / 40.9, 640 54.1 / 54.6.
+  p.narrow_join = (rows + 31) / 32 * ((hd + 15) / 16) * n_kv * n_seqs <= 4L * gi::sm_count();
   return p;
 }
 
@@ -477,9 +481,9 @@ extern "C" int gi_attn_tree(void* out, long ldo, const void* q, long ldq, long q
   if (rc != GI_OK) return rc;
   const int rows = max_nodes * (n_heads / n_kv);
   const int vec = hd % 8 == 0 && ldo % 8 == 0 && ((uintptr_t)out & 15) == 0;
-  const int numbers = p.many_parts ? 16 : 64;               // of a head, in a block of the join
+  const int numbers = p.narrow_join ? 16 : 64;               // of a head, in a block of the join
   const dim3 join((unsigned)((rows + 31) / 32 * ((hd + numbers - 1) / numbers)), n_kv, n_seqs);
-  GI_DISPATCH_DTYPE(dtype, T, rc = gi::check(gi::launch(p.many_parts ? attn_tree_join_kernel<T, 8> : attn_tree_join_kernel<T, 2>, join, dim3(THREADS), 0, s, sh, (T*)out,
+  GI_DISPATCH_DTYPE(dtype, T, rc = gi::check(gi::launch(p.narrow_join ? attn_tree_join_kernel<T, 8> : attn_tree_join_kernel<T, 2>, join, dim3(THREADS), 0, s, sh, (T*)out,
                                                         ldo, hd, p.ranges, tensor ? 1 : 0, vec, part_o, part_ml, prefix_out), "tree attention (join)"));
   return rc;
 }
