@@ -19,7 +19,8 @@
 // rows keeps all SMs busy, and leaves one list for every row it meets.  Tiles come through a ring in shared memory, which keeps
 // 96 KB an SM under way with few registers; with the next tile in registers instead, the kernel spilled and took twice as
 // long.  A warp fetches its columns of a tile in the aligned 16-byte pieces that hold them (of a row that starts between two
-// boundaries one more for every 32) and reads them by column.
+// boundaries one more for every 32) and reads them by column: 256 32-bit rows of
+// 128,255 tokens take 45 us for 43.5, 16-bit ones 43 for 40.
 // What enters a part's list must reach a bar that at least `width` of the part's logits reach.  The first bar is the smallest of
 // the warps' k-th largest lane maxima in the part's first tile, k = ceil(width / warps).  After the part's tiles 1, 4, 16, ... the list
 // is cut down to its `width` best and the bar raised to the last of them: each step then adds about 3 `width` entries.  A
@@ -91,6 +92,19 @@ template <> struct Piece<__nv_bfloat16> {
     }
   }
 };
+
+template <int N>
+__device__ __forceinline__ void load(unsigned* w, const unsigned* p) {
+  if constexpr (N == 4) {
+    const uint4 v = *reinterpret_cast<const uint4*>(p);
+    w[0] = v.x, w[1] = v.y, w[2] = v.z, w[3] = v.w;
+  } else if constexpr (N == 2) {
+    const uint2 v = *reinterpret_cast<const uint2*>(p);
+    w[0] = v.x, w[1] = v.y;
+  } else {
+    w[0] = *p;
+  }
+}
 
 // How the rows are cut, the same on both sides.
 struct Cut {
@@ -211,26 +225,50 @@ beam_rows_kernel(const T* logits, long ld, int vocab, int rows, Cut cut, int wid
     const unsigned off = (unsigned)(uintptr_t)(logits + (size_t)row * ld) & 15u;
     const unsigned char* from = (const unsigned char*)(ring + (here.stage * VPT * WARPS + warp) * WARP_PIECES + lane) + off;
     constexpr int STEP = WARPS * WARP_PIECES * 16;   // bytes from a thread's piece to its next one
+    const int turn = sizeof(T) == 4 && off != 0 ? lane >> 3 : 0;
+    auto behind = [&](int i) { return i / N * THREADS * N + (sizeof(T) == 4 ? (i + turn) & 3 : i % N); };      // x[i]'s token behind the first one's
     float x[NUMBERS];
     if (off == 0) {
 #pragma unroll
       for (int i = 0; i < VPT; ++i) Piece<T>::numbers(*reinterpret_cast<const uint4*>(from + i * STEP), x + i * N);
-    } else {
-      const unsigned turn = 8 * (off & 3u);           // 16-bit numbers that start in the middle of a word
+    } else if constexpr (sizeof(T) == 4) {
+      // word by word, every eight lanes in another order: words of one order lie in eight banks only
 #pragma unroll
-      for (int i = 0; i < VPT; ++i) {
-        const unsigned* w = reinterpret_cast<const unsigned*>(from - (off & 3u) + i * STEP);
-        uint4 v;
-        if (sizeof(T) == 4 || turn == 0) v = make_uint4(w[0], w[1], w[2], w[3]);
-        else v = make_uint4(__funnelshift_r(w[0], w[1], turn), __funnelshift_r(w[1], w[2], turn), __funnelshift_r(w[2], w[3], turn), __funnelshift_r(w[3], w[4], turn));
-        Piece<T>::numbers(v, x + i * N);
-      }
+      for (int e = 0; e < 4; ++e)
+#pragma unroll
+        for (int i = 0; i < VPT; ++i) x[i * N + e] = *reinterpret_cast<const float*>(from + ((e + turn) & 3) * 4 + i * STEP);
+    } else {
+      // the four words from word `words` of the piece on, and for a row that starts in the middle of a word the one behind them
+      auto from_two = [&](auto words) {
+        constexpr int W = decltype(words)::value;
+#pragma unroll
+        for (int i = 0; i < VPT; ++i) {
+          const unsigned* p = reinterpret_cast<const unsigned*>(from - off + i * STEP);
+          unsigned w[8];
+          if (W < 2) load<4>(w, p);
+          else if (W == 2) load<2>(w + 2, p + 2);
+          else load<1>(w + 3, p + 3);
+          constexpr int MORE = W + 1;
+          if (MORE == 1) load<1>(w + 4, p + 4);
+          else if (MORE == 2) load<2>(w + 4, p + 4);
+          else if (MORE > 2) load<4>(w + 4, p + 4);
+          if (off & 2u)
+            Piece<T>::numbers(make_uint4(__funnelshift_r(w[W], w[W + 1], 16), __funnelshift_r(w[W + 1], w[W + 2], 16), __funnelshift_r(w[W + 2], w[W + 3], 16),
+                                         __funnelshift_r(w[W + 3], w[W + 4], 16)), x + i * N);
+          else
+            Piece<T>::numbers(make_uint4(w[W], w[W + 1], w[W + 2], w[W + 3]), x + i * N);
+        }
+      };
+      if (off < 4) from_two(std::integral_constant<int, 0>());
+      else if (off < 8) from_two(std::integral_constant<int, 1>());
+      else if (off < 12) from_two(std::integral_constant<int, 2>());
+      else from_two(std::integral_constant<int, 3>());
     }
     const int token0 = (tile * VPT * THREADS + tid) * N;         // piece i's first token: THREADS * N further each
     if ((tile + 1) * (long)TILE > vocab) {
 #pragma unroll
       for (int i = 0; i < NUMBERS; ++i)
-        if (token0 + i / N * THREADS * N + i % N >= vocab) x[i] = -INFINITY;
+        if (token0 + behind(i) >= vocab) x[i] = -INFINITY;
     }
     float tops[2] = {-INFINITY, -INFINITY};           // (a maximum passes over what is no number)
 #pragma unroll
@@ -259,7 +297,9 @@ beam_rows_kernel(const T* logits, long ld, int vocab, int rows, Cut cut, int wid
           const float2 e = exp2_of(decltype(look)::value ? fmaxf(x[i], -INFINITY) : x[i], decltype(look)::value ? fmaxf(x[i + 1], -INFINITY) : x[i + 1], shift);
           more[i & 3] += e.x, more[(i & 3) + 1] += e.y;
         }
-        sum = (more[0] + more[1]) + (more[2] + more[3]);
+        // (back in the tokens' order: the sum is the same in every row)
+        const float a = turn & 1 ? more[3] : more[0], b = turn & 1 ? more[0] : more[1], c = turn & 1 ? more[1] : more[2], d = turn & 1 ? more[2] : more[3];
+        sum = turn & 2 ? (c + d) + (a + b) : (a + b) + (c + d);
 #pragma unroll
         for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
       };
@@ -279,8 +319,8 @@ beam_rows_kernel(const T* logits, long ld, int vocab, int rows, Cut cut, int wid
       while (hits != 0) {
         const int i = __ffs(hits) - 1;
         hits &= hits - 1;
-        const float v = gi::ldf(reinterpret_cast<const T*>(from + i / N * STEP) + i % N);
-        const u64 own = entry_of(v, token0 + i / N * THREADS * N + i % N);
+        const float v = gi::ldf(reinterpret_cast<const T*>(from + i / N * STEP) + (sizeof(T) == 4 ? (i + turn) & 3 : i % N));
+        const u64 own = entry_of(v, token0 + behind(i));
         if (own >= bar) {
           const int to = atomicAdd(&s.count, 1);
           if (to < CAP) s.list[to] = own;
