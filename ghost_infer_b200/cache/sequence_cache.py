@@ -131,6 +131,7 @@ class SequenceCache:
         self.slots = SlotAllocator(max_slots)
         self.max_slots = max_slots
         self.lengths = [0] * max_slots
+        self.turns = [0] * max_slots                   # counts up whenever what a slot holds, or where its next tokens go, may change
         self._groups: List[_Group] = []
         self._group_of_entry: Dict[int, Tuple[_Group, int]] = {}
         self._reads_from: Dict[int, int] = {}
@@ -183,6 +184,7 @@ class SequenceCache:
     def open_slot(self) -> int:
         s = self.slots.take()
         self.lengths[s] = 0
+        self.turns[s] += 1
         for g in self._groups:
             g.pages[s] = []
             g.first_live[s] = 0
@@ -225,6 +227,8 @@ class SequenceCache:
             if need > g.pool.free_pages:
                 raise CacheFullError(
                     f"the cache is full: {need} more pages of {PAGE_TOKENS} tokens wanted, {g.pool.free_pages} of {g.pool.n_pages} free")
+        for s, _ in wanted:
+            self.turns[s] += 1
         for g in self._groups:
             for s, n in wanted:
                 have = len(g.pages[s])
@@ -331,6 +335,7 @@ class SequenceCache:
                     self._mark(g, to, same, n)
         for to, src in moves:
             self.lengths[to] = was[src]
+            self.turns[to] += 1
         states = [t for d in (self._state, self._block_state) for t in d.values()]
         if not states:
             return
@@ -380,6 +385,7 @@ class SequenceCache:
             for t in d.values():
                 t[slot].zero_()
         self.lengths[slot] = 0
+        self.turns[slot] += 1
 
     def truncate(self, slot: int, pos: int) -> int:
         """Rewinds a slot to `pos` tokens (src/model.rs:799-821: lowering the position is enough for
@@ -388,6 +394,7 @@ class SequenceCache:
         cur = self.lengths[slot]
         if pos < cur and not (self._state or self._block_state or any(g.request.kind in ("window", "chunk") and g.first_live[slot] * PAGE_TOKENS > 0 for g in self._groups)):
             cur = self.lengths[slot] = pos
+        self.turns[slot] += 1
         keep = pages_for(cur)
         for g in self._groups:
             pages = g.pages[slot]

@@ -53,6 +53,7 @@ class TreeStep:
     logits: torch.Tensor
     context: "StepContext"
     entries: List[TreeEntry]
+    turns: List[int]                       # the cache's count for every entry's slot when the step ran
     done: bool = False
 
 
@@ -362,19 +363,19 @@ class Engine:
         self.bytes_h2d += packed.nbytes
         T = ctx.n_tokens
         ctx.tree = TreeFacts(dev[:T * words].view(T, words), dev[T * words:T * words + T], dev[T * words + T:])
-        return TreeStep(self.forward(ctx), ctx, list(entries))
+        return TreeStep(self.forward(ctx), ctx, list(entries), [self.cache.turns[e.slot] for e in entries])
 
     def commit_tree(self, tree: TreeStep, picks: torch.Tensor) -> List[List[int]]:
         """Takes over what the picks (int32 [nodes] on the device, in the order of the logits' rows: the token chosen after each
         node) agree with: from a tree's first node on, the child whose token is the pick, as long as there is one.  The slots then
-        hold the accepted tokens, and no pages but those they lie in.  Returns, for every entry, the accepted nodes' tokens after the first, and
+        hold the accepted tokens, and no pages but those they lie in.  Only a slot's latest step can be taken over.  Returns, for every entry, the accepted nodes' tokens after the first, and
         behind them the pick after the last one."""
         from ..kernels import ops
         if tree.done:
             raise RuntimeError("this step has been committed already")
         ctx = tree.context
-        for e, pos0 in zip(tree.entries, ctx.host_pos0):
-            if not self.cache.slots.live(e.slot) or self.cache.length(e.slot) != pos0:
+        for e, turn in zip(tree.entries, tree.turns):
+            if not self.cache.slots.live(e.slot) or self.cache.turns[e.slot] != turn:
                 raise RuntimeError(f"slot {e.slot} has moved on since this step")
         out = None
         for g in self.cache.groups:

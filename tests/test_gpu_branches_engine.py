@@ -92,6 +92,46 @@ def test_a_tree_step_that_is_not_committed_leaves_nothing(model_dirs, tiny_confi
         eng.commit_tree(dropped, torch.zeros(3, dtype=torch.int32, device="cuda:0"))
 
 
+def test_only_the_latest_step_over_trees_can_be_committed(model_dirs, tiny_configs):
+    """A step whose nodes' places were written again, given back or taken over by another sequence is refused, also where the slot
+    is as long as it was."""
+    d = model_dirs("A", "float32")
+    eng = make_engine(d, "float32")
+    prompt = tokens_for(tiny_configs["A"], 40, 1)
+    picks = torch.full((3,), 5, dtype=torch.int32, device="cuda:0")
+    s = eng.cache.open_slot()
+    eng.step([StepEntry(s, prompt)])
+
+    def drafted(tokens=(7, 5, 5)):
+        return eng.step_tree([TreeEntry(s, list(tokens), [-1, 0, 1])])
+
+    def again(step):
+        with pytest.raises(RuntimeError):
+            eng.commit_tree(step, picks)
+
+    first = drafted((1, 2, 3))
+    second = drafted()
+    again(first)                                        # another step over trees
+    eng.cache.truncate(s, 40)
+    again(second)                                       # its pages went back
+    third = drafted()
+    other = eng.cache.fork(s)
+    eng.cache.reorder([[s, other]], [[1, 0]])
+    again(third)                                        # the slot holds what another one held
+    fourth = drafted()
+    eng.cache.close_slot(s)
+    eng.cache.close_slot(other)
+    again(fourth)
+    s2 = eng.cache.open_slot()
+    eng.step([StepEntry(s2, prompt)])
+    assert s2 in (s, other)
+    s = s2
+    again(fourth)                                       # another sequence in the same slot
+    assert eng.commit_tree(drafted(), picks) == [[5, 5, 5]] and eng.cache.length(s) == 43
+    out = eng.step([StepEntry(s, [9], [0])]).cpu().numpy()
+    check_logits(out, plain_logits(d, prompt + [7, 5, 5, 9])[-1:], "float32")
+
+
 def test_trees_that_are_refused(model_dirs):
     eng = make_engine(model_dirs("A", "float32"), "float32")
     s = eng.cache.open_slot()
