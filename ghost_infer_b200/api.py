@@ -69,7 +69,9 @@ class LLM:
                     stop_token_ids: Optional[Sequence[int]] = None, batch_size: int = 1) -> List[List[BeamResult]]:
         """The `beams` (1 to 32) best continuations of every prompt that beam search finds, best first, `batch_size` prompts at a
         time.  Results are ordered by log probability / tokens ** length_penalty; a search ends when as many results have
-        ended as there are beams and nothing still going is more probable, or at `max_new` tokens."""
+        ended as there are beams and nothing still going is more probable than the `beams`-th most probable of them, or at `max_new`
+        tokens.  That end goes by log probability alone: with a penalty above zero a longer result may have had a better
+        score than those found, and is not looked for."""
         stop = self.stop_token_ids if stop_token_ids is None else stop_token_ids
         out = BeamSearch(self.engine, beams, stop, length_penalty, batch_size).run(prompts, max_new)
         self._check_kernels()
@@ -80,7 +82,8 @@ class LLM:
         """`generate` at temperature 0, several tokens a step where a draft is right.  `drafter(tokens, most)` gives at most `most`
         tokens that may follow and, for each, which of them it continues (-1: the last of `tokens`); None: `PromptLookup`, what
         followed the same words earlier in the sequence.  `max_nodes` (1 to 256): tokens a sequence runs in one step.  For models
-        that attend to all cached positions in every layer."""
+        that attend to all cached positions in every layer.  A step over trees is launched kernel by kernel where `generate` replays a
+        recording, so it takes several times as long: it pays where enough drafted tokens are right."""
         stop = self.stop_token_ids if stop_token_ids is None else stop_token_ids
         loop = DraftedLoop(self.engine, drafter if drafter is not None else PromptLookup(), stop, batch_size, max_nodes)
         results = loop.run(prompts, max_new)

@@ -11,8 +11,11 @@
 // head's group, which share every key and value that is read) and a range of tiles of 64 keys (attention_tree.cuh).  Scores are a
 // register tile of R / 16 rows by 4 keys a thread, sums of values R / 16 rows by 4 numbers for every 64 of the head; a row's 16
 // threads are one half of a warp, so its maximum and sum need no barrier.
+// Other head sizes come here in 16 bits too, for which the multiply-adds are far from what tensor cores do: 8 trees of 64 nodes behind
+// 8,192 positions, 32 heads over 8, take 1,811 us with heads of 80 and 1,926 with 96, where the tensor-core form takes 78 with heads of 64
+// and 88 with 128.
 // Bound: 32-bit multiply-adds (2 per query number and key) with many rows, the cache's bytes with few.  B200, 3 trees of 5 to 17
-// nodes behind 100 to 701 positions, 32 heads of 64 over 8: 20 us with the join (two tiles a block 30; breaks inside the inner loops
+// nodes behind 100 to 701 positions, 32 heads of 64 over 8: 20 to 23 us with the join (two tiles a block 30; breaks inside the inner loops
 // for rows that are not there 33; the body for 16 rows beside the one for 64 chosen by unit instead).
 #include <float.h>
 

@@ -19,7 +19,8 @@
 //
 // Bound: the cache's bytes with up to 128 rows (64 KB a tile at head size 128 take an SM's share of the memory about 2,850 cycles;
 // products take 1,200, the row threads 2,400), the row threads with more.  B200, 32 heads of 128 over 8, 8 sequences behind 8,192
-// positions: 1 node 56 us, 32 nodes 60 us (4.5 TB/s), 64 nodes 86 us (0.8 PFLOP/s).  Every wait has an iteration limit.
+// positions: 1 node 56 us, 32 nodes 60 us (4.5 TB/s), 64 nodes 88 us (0.78 PFLOP/s) for the first few hundred launches at 1,965 MHz; without
+// a pause the power limit brings the clock down to 1,580 MHz and 64 nodes to 106 us (0.65 PFLOP/s).  Every wait has an iteration limit.
 #include <cuda.h>
 
 #include "api.h"

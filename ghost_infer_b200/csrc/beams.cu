@@ -19,8 +19,8 @@
 // rows keeps all SMs busy, and leaves one list for every row it meets.  Tiles come through a ring in shared memory, which keeps
 // 96 KB an SM under way with few registers; with the next tile in registers instead, the kernel spilled and took twice as
 // long.  A warp fetches its columns of a tile in the aligned 16-byte pieces that hold them (of a row that starts between two
-// boundaries one more for every 32) and reads them by column: 256 32-bit rows of
-// 128,255 tokens take 45 us for 43.5, 16-bit ones 43 for 40.
+// boundaries one more for every 32) and reads them by column: 256 32-bit rows of 128,255 tokens take 45 us for 43.5 (fetched word by
+// word 60, four lanes at a time in the same banks 50), 16-bit ones 43 for 40.
 // What enters a part's list must reach a bar that at least `width` of the part's logits reach.  The first bar is the smallest of
 // the warps' k-th largest lane maxima in the part's first tile, k = ceil(width / warps).  After the part's tiles 1, 4, 16, ... the list
 // is cut down to its `width` best and the bar raised to the last of them: each step then adds about 3 `width` entries.  A
@@ -29,7 +29,7 @@
 // A piece whose sum is no number (a logit was none, or infinite) is added up once more with what is no number as -inf.
 // Bound: neither the memory (41 % of its rate) nor the issue slots (20 instructions a logit would fill them for 18 us), but what 20
 // warps an SM cannot hide: fixed latencies, the barriers around the lists, SMs that have two blocks and not three.  B200, 32
-// sequences of 8 beams over 128,256 tokens, 16 candidates: 43 us in all, the join a few of them; one sequence of 4 beams 9.4 us.
+// sequences of 8 beams over 128,256 tokens, 16 candidates: 43.5 us in all, the join a few of them; one sequence of 4 beams 9.5 us.
 #include <math.h>
 
 #include <type_traits>

@@ -9,8 +9,9 @@
 // Pages: the first `rows` positions of page src[i] are copied to page dst[i], for every layer and kv head.  A head's filled rows of
 // a page are one stretch of memory.
 //
-// Both are bound by the bytes they move: B200, states of 64 beams in 4 layers, 2 MB each, 88 us (6.2 TB/s); 128 pages of 28 layers, 8
-// kv heads of 128, half filled, 145 us (6.5 TB/s).
+// Both are bound by the bytes they move: B200, states of 8 sequences of 8 beams in 4 layers, 2 MB each, 88 us (6.2 TB/s); 128 pages of 28
+// layers, 8 kv heads of 128, half filled, 145 us (6.5 TB/s).  Not so above 16 beams, where shared memory leaves few columns to an SM: the
+// same states of 2 sequences of 32 beams take 305 us (1.8 TB/s), of one of 64 beams 372 us.
 #include "api.h"
 #include "common.cuh"
 #include "page_tensors.cuh"

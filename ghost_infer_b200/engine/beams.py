@@ -5,7 +5,8 @@ there are beams (pages are shared, see `SequenceCache.fork`), and every step is:
 2 x beams (or more) best of beams x vocabulary (`ops.beam_select`), the ones among them that end the sequence set aside, the others'
 first `beams` fed next after the cache has followed them (`SequenceCache.reorder`).  Twice as many candidates as beams leave
 enough that do not end: a beam has a candidate that ends for each of the stop tokens.  More stop tokens ask for more candidates, as
-many as `ops.beam_select` gives (64); where all of those were ends, fewer beams would go on.
+many as `ops.beam_select` gives (64); where all of those were ends, fewer beams would go on.  The end of a search goes by log
+probability, not by the score that orders results: the score of a beam that goes on still changes with its length.
 """
 from __future__ import annotations
 
